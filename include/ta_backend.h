@@ -93,6 +93,108 @@ int ta_silu_mul_bwd(const uint16_t* dout, const uint16_t* gate, const uint16_t* 
 int ta_cross_entropy_fwd(const uint16_t* logits, const int32_t* targets, float* loss_out,
                          uint16_t* dlogits, int N, int V, void* stream);
 
+/* ── token log-probabilities ─────────────────────────────────────────
+ * No counterpart in the reference, whose only loss is the cross entropy.
+ * What preference and policy losses are made of: for each row of V logits l,
+ * with x = inv_temp * l (inv_temp > 0: the inverse sampling temperature) and
+ * the row's token t = targets[row],
+ *   lse = log sum_v exp(x_v),  logp = x_t - lse,
+ *   entropy = -sum_v p_v log p_v  (p = exp(x - lse); may be NULL).
+ * logits: rows of V values, ld elements apart (ld >= V), at any alignment of
+ * their type.  A row with t < 0 has no token: its logits are not read and its
+ * three results are 0.  A row with t >= V, a NaN, a +Inf or nothing above
+ * -Inf gives NaN; single logits of -Inf have p = 0.  All sums are F32. */
+int ta_token_logp_fwd(const uint16_t* logits, int64_t ld, const int32_t* targets, float inv_temp,
+                      float* logp, float* lse, float* entropy, int N, int V, void* stream);
+int ta_token_logp_fwd_f32(const float* logits, int64_t ld, const int32_t* targets, float inv_temp,
+                          float* logp, float* lse, float* entropy, int N, int V, void* stream);
+
+/* Gradient of ta_token_logp_fwd, from the lse (and, with dentropy, the
+ * entropy) it gave:
+ *   dlogits_v = inv_temp (dlogp ([v = t] - p_v) - dentropy p_v (log p_v + entropy)),
+ * rounded once to the logits' type, rows ldd elements apart; dentropy may be
+ * NULL (then entropy may be too).  Rows without a token, and rows whose dlogp
+ * and dentropy are 0, get zeros and are not read.  dlogits may be logits
+ * itself (with ldd = ld).  p comes from the F32 lse: |x| beyond 2^20 leaves
+ * it no digits. */
+int ta_token_logp_bwd(const uint16_t* logits, int64_t ld, const int32_t* targets, float inv_temp,
+                      const float* lse, const float* entropy, const float* dlogp,
+                      const float* dentropy, uint16_t* dlogits, int64_t ldd, int N, int V,
+                      void* stream);
+int ta_token_logp_bwd_f32(const float* logits, int64_t ld, const int32_t* targets, float inv_temp,
+                          const float* lse, const float* entropy, const float* dlogp,
+                          const float* dentropy, float* dlogits, int64_t ldd, int N, int V,
+                          void* stream);
+
+/* ta_token_logp_fwd of the logits h W^T, which are never stored: for scoring
+ * by the frozen base or by an old policy, where no gradient follows.
+ * h [N, H] (row stride ldh) and W [V, H] (row stride ldw) BF16.  round_logits
+ * 1 rounds each logit to BF16 first, as ta_gemm_bf16 writes it, so the result
+ * is that of ta_token_logp_fwd on those logits up to the order of sums; 0
+ * keeps them in F32.  ws: ta_lm_head_logp_ws(N, V) bytes of the caller's for
+ * this call alone, or NULL: the stream's scratch pool.  Rows without a token
+ * give 0 (their logits are still computed).  No reference counterpart. */
+int ta_lm_head_logp(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t ldw,
+                    const int32_t* targets, float inv_temp, int round_logits, float* logp,
+                    float* lse, float* entropy, int N, int V, int H, void* ws, void* stream);
+int64_t ta_lm_head_logp_ws(int N, int V);
+
+/* ── preference loss ──────────────────────────────────────────────────
+ * No reference counterpart.  P pairs of packed sequences: sequence 2p is the
+ * chosen answer of pair p, 2p + 1 the rejected one; sequence q holds the
+ * tokens offsets[q] .. offsets[q + 1] - 1 (offsets: device int64 [2P + 1],
+ * taken within 0 .. N) of the token arrays, of which those with target >= 0
+ * count.  With pi_q and ref_q the sums of logp and ref_logp over the counting
+ * tokens of q (their means if average is 1; ref_logp NULL: 0) and
+ * u = (pi_2p - pi_2p+1) - (ref_2p - ref_2p+1), z = beta u - margin:
+ *   TA_PREF_SIGMOID  (1 - smoothing) softplus(-z) + smoothing softplus(z)
+ *   TA_PREF_IPO      (u - margin - 1 / (2 beta))^2
+ *   TA_PREF_HINGE    max(0, 1 - z)
+ * pair_loss [P] gets the pair's loss, rewards [P][2] (may be NULL)
+ * beta (pi - ref) of both answers, dlogp (may be NULL) the gradient of
+ * scale * sum of the pair losses to each token's logp (1/P for their mean).
+ * A pair of which one answer has no counting token takes no part: loss 0, no
+ * gradient.  Tokens that do not count get gradient 0, tokens of no sequence
+ * are left as they were.  Sums and the loss are formed in 64 bits. */
+enum { TA_PREF_SIGMOID = 0, TA_PREF_IPO = 1, TA_PREF_HINGE = 2 };
+int ta_preference_loss(const float* logp, const float* ref_logp, const int32_t* targets,
+                       const int64_t* offsets, int P, int64_t N, int kind, int average, float beta,
+                       float smoothing, float margin, float scale, float* pair_loss,
+                       float* rewards, float* dlogp, void* stream);
+
+/* ── clipped policy loss ──────────────────────────────────────────────
+ * No reference counterpart.  For each of N tokens with the advantage A, with
+ * r = exp(logp - old_logp) (old_logp NULL: the policy itself, r = 1) and
+ * d = ref_logp - logp (ref_logp NULL: no KL term):
+ *   pg   = -min(r A, clip(r, 1 - clip_lo, 1 + clip_hi) A), and for A < 0
+ *          with dual_clip > 1 (0: off) min(pg, -dual_clip A)
+ *   kl   = exp(d) - d - 1
+ *   loss = pg + kl_beta kl
+ * loss and kl (each may be NULL) get the token's values, dlogp the gradient
+ * of the sum of weight * loss.  weight: 1 / tokens for the mean of the batch,
+ * 1 / (sequences * tokens of the sequence) for the mean of sequence means; a
+ * token of weight 0 is masked: its outputs are 0 and nothing else of it is
+ * used.  logp - old_logp and d are taken within +-60, past which the loss
+ * counts as flat in them. */
+int ta_policy_loss(const float* logp, const float* old_logp, const float* ref_logp,
+                   const float* adv, const float* weight, float clip_lo, float clip_hi,
+                   float dual_clip, float kl_beta, float* loss, float* kl, float* dlogp,
+                   int64_t N, void* stream);
+
+/* The same from the logits to their gradient in one pass over them:
+ * ta_token_logp_fwd, ta_policy_loss with the entropy bonus
+ * loss = pg + kl_beta kl - ent_coef entropy, and ta_token_logp_bwd of both
+ * terms.  Rows without a token (t < 0 or weight 0) are not read; their
+ * results and gradient are 0.  logp, entropy (may be NULL when ent_coef is 0)
+ * and kl (may be NULL) get the row's values; dlogits may be logits itself
+ * (with ldd = ld). */
+int ta_policy_loss_logits(const uint16_t* logits, int64_t ld, const int32_t* targets,
+                          float inv_temp, const float* old_logp, const float* ref_logp,
+                          const float* adv, const float* weight, float clip_lo, float clip_hi,
+                          float dual_clip, float kl_beta, float ent_coef, float* logp,
+                          float* entropy, float* loss, float* kl, uint16_t* dlogits, int64_t ldd,
+                          int N, int V, void* stream);
+
 /* ── embedding ──────────────────────────────────────────────────────
  * replaces ops::embed_fwd / embed_bwd  ops.hpp:98-110 (ops.cu:1026-1051).
  * embed_bwd accumulates (+=) into the F32 dtable with atomics, as the

@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "lds_tr.hpp"
+#include "soft.hpp"
 #include "ta_backend.h"
 #include "ta_internal.hpp"
 
@@ -50,7 +51,8 @@ __device__ __forceinline__ void st_out16(void* p, const bf16x8v& v) {
 constexpr int BK = 64;
 constexpr int LDS_STRIDE = BK + 8;  // bf16 elements per LDS row
 
-enum Epi { EPI_BF16 = 0, EPI_PARTIAL = 2 };
+// EPI_LSE: the row statistics of lse_tile instead of C
+enum Epi { EPI_BF16 = 0, EPI_PARTIAL = 2, EPI_LSE = 3 };
 
 struct GemmArgs {
     int M, N, K;
@@ -192,6 +194,82 @@ struct TileLoader {
     }
 };
 
+// Softmax statistics of one tile (ta_lm_head_logp): the logits are the
+// accumulators, transposed (Y rows as the MFMA's A operand): lane l of
+// acc[i][j] has row 32i + l%32 and columns 32j + 8(r/4) + 4(l/32) + r%4.  Each
+// row's (m, s, u) over the tile's columns goes to part [tiles_n][3][M], the
+// logit of the row's token, where this tile has it, to C [M].  Arguments in
+// the fields this form has free: ce_tgt the tokens, ce_inv_n = inv_temp
+// log2(e), lora_r bit 0: logits rounded to BF16 first, bit 1: u too.
+// A lane holds a row's 16 TN columns of its wave, the lane 32 on the others;
+// the WNW waves of a row meet in red (LDS, [WNW][BM]).
+template <int TM, int TN, int BM, int WNW, int NT>
+__device__ __forceinline__ void lse_tile(floatx16 (&acc)[TM][TN], const GemmArgs& a, int m0,
+                                         int n0, int wrow, int wn, int tn_i, int lane,
+                                         Soft* red) {
+    const int c0 = n0 + wn * TN * 32, c4 = 4 * (lane >> 5);
+    const float c2 = a.ce_inv_n;
+    const bool round = (a.lora_r & 1) != 0, ent = (a.lora_r & 2) != 0;
+    const bool tail = n0 + WNW * TN * 32 > a.N;  // (uniform) columns past N hold no logit
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const int row = m0 + wrow + 32 * i + (lane & 31);
+        if (round) {
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) acc[i][j][r] = bf2f(f2bf(acc[i][j][r]));
+        }
+        const int t = row < a.M ? a.ce_tgt[row] : -1;
+        if (t >= c0 && t < min(c0 + TN * 32, a.N)) {
+            float ft = 0.f;
+            bool mine = false;
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (c0 + 32 * j + 8 * (r >> 2) + c4 + (r & 3) == t) ft = acc[i][j][r], mine = true;
+            if (mine) ((float*)a.C)[row] = ft;
+        }
+        if (tail) {
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (c0 + 32 * j + 8 * (r >> 2) + c4 + (r & 3) >= a.N) acc[i][j][r] = -INFINITY;
+        }
+        Soft st = {-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) st.m = fmaxf(st.m, acc[i][j][r]);
+        st.m = fmaxf(st.m, __shfl_xor(st.m, 32, 64));
+        const float R = soft_ref(st.m);
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float d = acc[i][j][r] - R, p = __builtin_amdgcn_exp2f(d * c2);
+                st.s += p;
+                if (ent) st.u = fmaf(p, fmaxf(d, kFar), st.u);
+            }
+        st.s += __shfl_xor(st.s, 32, 64);
+        st.u += __shfl_xor(st.u, 32, 64);
+        if (lane < 32) red[wn * BM + wrow + 32 * i + lane] = st;
+    }
+    __syncthreads();
+    for (int q = threadIdx.x; q < BM; q += NT) {
+        if (m0 + q >= a.M) break;
+        Soft st = red[q];
+#pragma unroll
+        for (int k = 1; k < WNW; k++) st = soft_merge(st, red[k * BM + q], c2);
+        float* P = a.part + (int64_t)tn_i * 3 * a.M + m0 + q;
+        P[0] = st.m;
+        P[a.M] = st.s;
+        P[2 * (int64_t)a.M] = st.u;
+    }
+}
+
 template <int BM, int BN, int WM, int WN, bool XK, bool YK, int EPI>
 __global__ __launch_bounds__(256) void k_gemm(GemmArgs a, bool vecx, bool vecy) {
     constexpr int WTM = BM / WM, WTN = BN / WN;  // wave tile
@@ -254,8 +332,12 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a, bool vecx, bool vecy) 
             for (int i = 0; i < TM; i++)
 #pragma unroll
                 for (int j = 0; j < TN; j++)
-                    acc[i][j] =
-                        __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx[i], fy[j], acc[i][j], 0, 0, 0);
+                    if constexpr (EPI == EPI_LSE)  // transposed accumulators (lse_tile)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fy[j], fx[i],
+                                                                            acc[i][j], 0, 0, 0);
+                    else
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fx[i], fy[j],
+                                                                            acc[i][j], 0, 0, 0);
         }
         if (more) {
             lx.store(sX[cur ^ 1]);
@@ -264,6 +346,12 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a, bool vecx, bool vecy) 
         __syncthreads();
     }
 
+    if constexpr (EPI == EPI_LSE) {
+        static_assert(BM * WN * sizeof(Soft) <= sizeof(sX), "row statistics fit the stages");
+        // (the last k-tile's barrier is behind every read of the stages)
+        lse_tile<TM, TN, BM, WN, 256>(acc, a, m0, n0, wm * WTM, wn, tn_i, lane, (Soft*)sX);
+        return;
+    }
     // epilogue: lane holds column n = lane%32 of each 32x32 tile and rows
     // 8*(r/4) + 4*(lane/32) + r%4
 #pragma unroll
@@ -2954,6 +3042,73 @@ int gemm_swiglu(int M, int K, const bf16* X, int64_t ldx, const bf16* Wgu, const
     return check_launch("gemm_swiglu");
 }
 
+// (m, s, u) of every row over the column tiles, then its results.  One block
+// per 64 rows, a row per lane: wave w takes tiles w, w + 16, .., whose rows
+// lie side by side.
+__global__ __launch_bounds__(1024) void k_lse_merge(const float* __restrict__ part, int tiles,
+                                                    const float* __restrict__ tlogit,
+                                                    const int32_t* __restrict__ targets, float c,
+                                                    float* __restrict__ logp,
+                                                    float* __restrict__ lse,
+                                                    float* __restrict__ entropy, int N, int V) {
+    __shared__ Soft red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int row = blockIdx.x * 64 + lane, rd = min(row, N - 1);
+    const float c2 = c * kLog2e;
+    Soft st = {-INFINITY, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = w; k < tiles; k += 16) {
+        const float* P = part + (int64_t)k * 3 * N + rd;
+        st = soft_merge(st, Soft{P[0], P[N], P[2 * (int64_t)N]}, c2);
+    }
+    red[w][lane] = st;
+    __syncthreads();
+    if (w != 0 || row >= N) return;
+#pragma unroll
+    for (int k = 1; k < 16; k++) st = soft_merge(st, red[k][lane], c2);
+    const int t = targets[row];
+    RowOut o = {0.f, 0.f, 0.f};
+    if (t >= 0) o = row_out(st, t < V ? tlogit[row] : 0.f, t < V, c);
+    logp[row] = o.logp;
+    lse[row] = o.lse;
+    if (entropy) entropy[row] = o.ent;
+}
+
+// bytes of partial statistics and token logits: no form has tiles narrower
+// than 128 columns
+int64_t lm_head_logp_ws(int N, int V) {
+    return ((int64_t)((V + 127) / 128) * 3 + 1) * N * (int64_t)sizeof(float);
+}
+
+int lm_head_logp(const bf16* h, int64_t ldh, const bf16* W, int64_t ldw, const int32_t* targets,
+                 float c, bool round, float* logp, float* lse, float* entropy, int N, int V, int H,
+                 void* ws, hipStream_t s) {
+    GemmArgs a{};
+    a.M = N;
+    a.N = V;
+    a.K = H;
+    a.X = h;
+    a.ldx = ldh;
+    a.Y = W;
+    a.ldy = ldw;
+    a.k_per_split = H;
+    a.ngroups = a.nseg = 1;
+    a.ce_tgt = targets;
+    a.ce_inv_n = c * kLog2e;
+    a.lora_r = (round ? 1 : 0) | (entropy ? 2 : 0);
+    if (!ws) ws = scratch_get((size_t)lm_head_logp_ws(N, V), s);
+    if (!ws) return set_error(-2, "lm_head_logp: scratch allocation failed");
+    a.C = ws;
+    a.part = (float*)ws + N;
+    a.tiles_m = (N + 127) / 128;
+    a.tiles_n = (V + 127) / 128;
+    tlaunch(k_gemm<128, 128, 2, 2, true, true, EPI_LSE>, dim3(a.tiles_m * a.tiles_n), dim3(256), s,
+            a, al16(h) && ldh % 8 == 0, al16(W) && ldw % 8 == 0);
+    tlaunch(k_lse_merge, dim3((N + 63) / 64), dim3(1024), s, a.part, a.tiles_n, (const float*)a.C,
+            targets, c, logp, lse, entropy, N, V);
+    return check_launch("lm_head_logp");
+}
+
 int gemm_ce_dx(int M, int N, int K, const bf16* logits, const bf16* Wt, bf16* C,
                const float* lse2, const int32_t* tgt, float inv_n, hipStream_t s) {
     TA_REQUIRE(M >= 256 && N >= 192 && K % BK == 0 && al16(logits) && al16(Wt) && al16(C) &&
@@ -3002,6 +3157,29 @@ int ta_gemm_rm(int x_kmajor, int y_kmajor, int M, int N, int K, float alpha, con
                "gemm_rm: M/N/K and leading dims must be > 0");
     return gemm_dispatch(x_kmajor != 0, y_kmajor != 0, M, N, K, alpha, X, ldx, Y, ldy, beta, C,
                          ldc, bias, (hipStream_t)stream, 0, nullptr);
+}
+
+int64_t ta_lm_head_logp_ws(int N, int V) {
+    return N > 0 && V > 0 ? lm_head_logp_ws(N, V) : 0;
+}
+
+int ta_lm_head_logp(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t ldw,
+                    const int32_t* targets, float inv_temp, int round_logits, float* logp,
+                    float* lse, float* entropy, int N, int V, int H, void* ws, void* stream) {
+    TA_REQUIRE(N >= 0 && V > 0 && H > 0 && ldh >= H && ldw >= H,
+               "lm_head_logp: bad shape N=%d V=%d H=%d ldh=%lld ldw=%lld", N, V, H,
+               (long long)ldh, (long long)ldw);
+    TA_REQUIRE(inv_temp > 0.f && inv_temp < INFINITY,
+               "lm_head_logp: inv_temp must be positive and finite");
+    TA_REQUIRE(round_logits == 0 || round_logits == 1, "lm_head_logp: round_logits must be 0 or 1");
+    TA_REQUIRE(V <= INT32_MAX - 256 && ((int64_t)N + 127) / 128 * ((V + 127) / 128) < (1 << 23),
+               "lm_head_logp: N=%d x V=%d takes more tiles than a launch", N, V);
+    if (N == 0) return 0;
+    TA_REQUIRE(h && W && targets && logp && lse, "lm_head_logp: null argument");
+    TA_REQUIRE((((uintptr_t)h | (uintptr_t)W) & 1) == 0 && ((uintptr_t)ws & 15) == 0,
+               "lm_head_logp: misaligned operand");
+    return lm_head_logp(h, ldh, W, ldw, targets, inv_temp, round_logits != 0, logp, lse, entropy, N,
+                        V, H, ws, (hipStream_t)stream);
 }
 
 int ta_gemm_plan(int M, int N, int K, int lora, int beta, int captured, int32_t* out) {

@@ -150,7 +150,7 @@ int64_t ta_lm_head_logp_ws(int N, int V);
  *   TA_PREF_SIGMOID  (1 - smoothing) softplus(-z) + smoothing softplus(z)
  *   TA_PREF_IPO      (u - margin - 1 / (2 beta))^2
  *   TA_PREF_HINGE    max(0, 1 - z)
- * pair_loss [P] gets the pair's loss, rewards [P][2] (may be NULL)
+ * (smoothing, in [0, 1), has no part in the last two).  pair_loss [P] gets the pair's loss, rewards [P][2] (may be NULL)
  * beta (pi - ref) of both answers, dlogp (may be NULL) the gradient of
  * scale * sum of the pair losses to each token's logp (1/P for their mean).
  * A pair of which one answer has no counting token takes no part: loss 0, no

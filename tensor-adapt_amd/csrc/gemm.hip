@@ -1282,17 +1282,20 @@ __device__ __forceinline__ void ce_frags(bf16x8_t (&fa)[TM], int kt, int kk, con
 // CEX: X holds logits and the MFMAs take dlogits formed from them (ce_frags).
 // PART: split-K, split blockIdx.z over k [z k_per_split, +k_per_split): F32
 // partials of the split into part[z][M][N], no epilogue arithmetic.
+// LSE: row statistics of the tile instead of C (lse_tile).
 // DEEP: 128-row tiles with DEEP stages of 64 k in flight, loaded by PW waves
 // of their own (0: the two-stage loop, loaded by the computing waves); see
 // k_gemm_deep.
 template <int BN, int WMW, int WNW, bool CHAIN, bool SWIGLU = false, int KD = 32, int BM = 256,
-          bool CEX = false, bool PART = false, int DEEP = 0, int PW = 0, bool YT = false>
+          bool CEX = false, bool PART = false, int DEEP = 0, int PW = 0, bool YT = false,
+          bool LSE = false>
 __device__ __attribute__((always_inline)) inline void gemm_pipe_body(const GemmArgs& a0) {
     static_assert(!CEX || (KD == 64 && !CHAIN && !SWIGLU), "CE operand form");
     static_assert(!PART || (KD == 64 && !CHAIN && !SWIGLU && !CEX), "split-K partials form");
     static_assert(KD == 32 || KD == 64, "stage depth");
     static_assert(DEEP == 0 || (KD == 64 && BM == 128 && !SWIGLU && !CEX), "deep form");
     static_assert(!YT || (DEEP > 0 && !CHAIN), "K-strided Y: deep form only");
+    static_assert(!LSE || (!CHAIN && !SWIGLU && !CEX && !PART), "row statistics form");
     constexpr int NS = DEEP ? DEEP : KD == 32 ? 4 : 2, NW = WMW * WNW;
     constexpr int LW = DEEP ? PW : NW;  // waves that load the stages
     constexpr int WTM = BM / WMW, WTN = BN / WNW;
@@ -1691,6 +1694,12 @@ __device__ __attribute__((always_inline)) inline void gemm_pipe_body(const GemmA
         }
         return;
     }
+    if constexpr (LSE) {
+        static_assert(BM * WNW * sizeof(Soft) <= sizeof(sXs), "row statistics fit the stages");
+        __syncthreads();  // every wave is done with the stage buffers
+        lse_tile<TM, TN, BM, WNW, NW * 64>(acc, a, m0, n0, wm * WTM, wn, tn_i, lane, (Soft*)sXs);
+        return;
+    }
 #undef PIPE_CE
 #undef PIPE_ROUND
 #undef PIPE_ISSUE
@@ -1803,6 +1812,17 @@ template <int BN, int WMW, int WNW>
 __global__ __launch_bounds__(WMW * WNW * 64) __attribute__((amdgpu_waves_per_eu(
     WMW * WNW / 4, WMW * WNW / 4))) void k_gemm_pipe_ce(GemmArgs a) {
     gemm_pipe_body<BN, WMW, WNW, false, false, 64, 256, true>(a);
+}
+// Row statistics of h W^T (ta_lm_head_logp) in 256 x 256 and 128 x 128 tiles.
+template <int BN, int WMW, int WNW>
+__global__ __launch_bounds__(WMW * WNW * 64) __attribute__((amdgpu_waves_per_eu(
+    WMW * WNW / 4, WMW * WNW / 4))) void k_gemm_pipe_lse(GemmArgs a) {
+    gemm_pipe_body<BN, WMW, WNW, false, false, 64, 256, false, false, 0, 0, false, true>(a);
+}
+template <int BN>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_gemm_mid_lse(
+    GemmArgs a) {
+    gemm_pipe_body<BN, 2, 2, false, false, 64, 128, false, false, 0, 0, false, true>(a);
 }
 // 128-row tiles (128 x BN, BN = 64 or 128; four waves of 64-row wave tiles,
 // two 64-k stages): the same pipeline and epilogue for outputs too small to
@@ -2129,7 +2149,7 @@ static const char* mid_name(int bn, bool chain) {
 }
 
 // whether s records into a graph (also when that cannot be told)
-static bool is_capturing(hipStream_t s) {
+bool is_capturing(hipStream_t s) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(s, &st) != hipSuccess) {
         (void)hipGetLastError();
@@ -3042,34 +3062,71 @@ int gemm_swiglu(int M, int K, const bf16* X, int64_t ldx, const bf16* Wgu, const
     return check_launch("gemm_swiglu");
 }
 
-// (m, s, u) of every row over the column tiles, then its results.  One block
-// per 64 rows, a row per lane: wave w takes tiles w, w + 16, .., whose rows
-// lie side by side.
+// (m, s, u) of every row over the column tiles, then its results.  A block
+// takes R rows, side by side in the partials, with 1024 / R lanes of tiles
+// each; a lane loads four tiles at a time and keeps its sums in 64 bits.
+template <int R>
 __global__ __launch_bounds__(1024) void k_lse_merge(const float* __restrict__ part, int tiles,
                                                     const float* __restrict__ tlogit,
                                                     const int32_t* __restrict__ targets, float c,
                                                     float* __restrict__ logp,
                                                     float* __restrict__ lse,
                                                     float* __restrict__ entropy, int N, int V) {
-    __shared__ Soft red[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int row = blockIdx.x * 64 + lane, rd = min(row, N - 1);
+    constexpr int LPR = 1024 / R, U = 4;
+    __shared__ float redm[16][R];
+    __shared__ double red[16][R][2];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = threadIdx.x % R;
+    const int64_t row = blockIdx.x * (int64_t)R + q, rd = min(row, (int64_t)N - 1);
+    const int64_t plane = N, tile = 3 * plane;
     const float c2 = c * kLog2e;
-    Soft st = {-INFINITY, 0.f, 0.f};
-#pragma unroll 4
-    for (int k = w; k < tiles; k += 16) {
-        const float* P = part + (int64_t)k * 3 * N + rd;
-        st = soft_merge(st, Soft{P[0], P[N], P[2 * (int64_t)N]}, c2);
-    }
-    red[w][lane] = st;
-    __syncthreads();
-    if (w != 0 || row >= N) return;
+    float m = -INFINITY;
+    double s = 0.0, u = 0.0;
+    for (int k0 = threadIdx.x / R; k0 < tiles; k0 += LPR * U) {
+        float tm[U], ts[U], tu[U], M = m;
 #pragma unroll
-    for (int k = 1; k < 16; k++) st = soft_merge(st, red[k][lane], c2);
+        for (int i = 0; i < U; i++) {
+            const int k = k0 + i * LPR;
+            const float* p = part + min(k, tiles - 1) * tile + rd;
+            tm[i] = k < tiles ? p[0] : -INFINITY;
+            ts[i] = k < tiles ? p[plane] : 0.f;
+            tu[i] = entropy && k < tiles ? p[2 * plane] : 0.f;
+            M = fmaxf(M, tm[i]);
+        }
+        const float g = soft_ref(M), dm = m - g, fm = __builtin_amdgcn_exp2f(dm * c2);
+        u = (double)fm * (u + s * (double)fmaxf(dm, kFar));
+        s *= (double)fm;
+        m = M;
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const float d = tm[i] - g, f = __builtin_amdgcn_exp2f(d * c2);
+            s += (double)(ts[i] * f);
+            u += (double)(f * (tu[i] + ts[i] * fmaxf(d, kFar)));
+        }
+    }
+    float M = m;
+#pragma unroll
+    for (int o = R; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    if (lane < R) redm[w][q] = M;
+    __syncthreads();
+    M = redm[0][q];
+#pragma unroll
+    for (int k = 1; k < 16; k++) M = fmaxf(M, redm[k][q]);
+    const float d = m - soft_ref(M);
+    const double f = (double)__builtin_amdgcn_exp2f(d * c2);
+    u = f * (u + s * (double)fmaxf(d, kFar));
+    s *= f;
+#pragma unroll
+    for (int o = R; o < 64; o <<= 1) s += __shfl_xor(s, o, 64), u += __shfl_xor(u, o, 64);
+    if (lane < R) red[w][q][0] = s, red[w][q][1] = u;
+    __syncthreads();
+    if (threadIdx.x >= R || row >= N) return;
+    SoftRow st = {M, red[0][q][0], red[0][q][1]};
+#pragma unroll
+    for (int k = 1; k < 16; k++) st.s += red[k][q][0], st.u += red[k][q][1];
     const int t = targets[row];
-    RowOut o = {0.f, 0.f, 0.f};
+    RowOut o = {0.0, 0.f, 0.f};
     if (t >= 0) o = row_out(st, t < V ? tlogit[row] : 0.f, t < V, c);
-    logp[row] = o.logp;
+    logp[row] = (float)o.logp;
     lse[row] = o.lse;
     if (entropy) entropy[row] = o.ent;
 }
@@ -3100,12 +3157,27 @@ int lm_head_logp(const bf16* h, int64_t ldh, const bf16* W, int64_t ldw, const i
     if (!ws) return set_error(-2, "lm_head_logp: scratch allocation failed");
     a.C = ws;
     a.part = (float*)ws + N;
-    a.tiles_m = (N + 127) / 128;
-    a.tiles_n = (V + 127) / 128;
-    tlaunch(k_gemm<128, 128, 2, 2, true, true, EPI_LSE>, dim3(a.tiles_m * a.tiles_n), dim3(256), s,
-            a, al16(h) && ldh % 8 == 0, al16(W) && ldw % 8 == 0);
-    tlaunch(k_lse_merge, dim3((N + 63) / 64), dim3(1024), s, a.part, a.tiles_n, (const float*)a.C,
-            targets, c, logp, lse, entropy, N, V);
+    const bool vx = al16(h) && ldh % 8 == 0, vw = al16(W) && ldw % 8 == 0;
+    const bool pipe = H % BK == 0 && vx && vw && ldh < kMaxStageLd && ldw < kMaxStageLd;
+    // 256-row tiles where 128-row ones would read W twice (151,936 x 1536, us:
+    // 128 rows 133 against 150, 129 rows 159 against 151, 256 rows 184 against
+    // 164, 8192 rows 3820 against 3170)
+    const int bt = pipe && N > 128 ? 256 : 128;
+    a.tiles_m = (N + bt - 1) / bt;
+    a.tiles_n = (V + bt - 1) / bt;
+    const dim3 grid(a.tiles_m * a.tiles_n);
+    if (bt == 256)
+        tlaunch(k_gemm_pipe_lse<256, 2, 4>, grid, dim3(512), s, a);
+    else if (pipe)
+        tlaunch(k_gemm_mid_lse<128>, grid, dim3(256), s, a);
+    else
+        tlaunch(k_gemm<128, 128, 2, 2, true, true, EPI_LSE>, grid, dim3(256), s, a, vx, vw);
+    if (N <= 1024)
+        tlaunch(k_lse_merge<4>, dim3((N + 3) / 4), dim3(1024), s, a.part, a.tiles_n,
+                (const float*)a.C, targets, c, logp, lse, entropy, N, V);
+    else
+        tlaunch(k_lse_merge<16>, dim3((unsigned)(((int64_t)N + 15) / 16)), dim3(1024), s, a.part,
+                a.tiles_n, (const float*)a.C, targets, c, logp, lse, entropy, N, V);
     return check_launch("lm_head_logp");
 }
 

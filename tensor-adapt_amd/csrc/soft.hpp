@@ -48,31 +48,93 @@ __device__ __forceinline__ void soft_add(Soft& st, const float* f, float c2) {
         if (ENT) st.u = fmaf(p, fmaxf(d, kFar), st.u);
     }
 }
+// Row statistics: S and U in 64 bits, since a sequence adds up the errors of
+// its rows' log S and the KL term divides them by small differences.
+struct SoftRow {
+    float m;
+    double s, u;
+};
+// A block's maximum and sums, for every thread (redm, red: LDS, one entry per
+// wave; one barrier each).  NW (a power of two) lanes read the waves' entries
+// and a butterfly joins them: every lane reading all of them takes 64
+// registers, which a row held in registers spills for.
 template <int NW>
-__device__ __forceinline__ Soft soft_block(Soft st, float c2, Soft* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const Soft b = {__shfl_xor(st.m, o, 64), __shfl_xor(st.s, o, 64), __shfl_xor(st.u, o, 64)};
-        st = soft_merge(st, b, c2);
-    }
-    __syncthreads();  // red is free
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = st;
+__device__ __forceinline__ float block_maxf(float m, float* redm) {
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) redm[threadIdx.x >> 6] = m;
     __syncthreads();
-    st = red[0];
+    m = redm[threadIdx.x & (NW - 1)];
 #pragma unroll
-    for (int k = 1; k < NW; k++) st = soft_merge(st, red[k], c2);
-    return st;
+    for (int o = NW / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    return m;
+}
+template <int NW, bool ENT>
+__device__ __forceinline__ SoftRow block_sums(float m, float s1, float u1, double (*red)[2]) {
+    const double s = wave_sum_d((double)s1), u = ENT ? wave_sum_d((double)u1) : 0.0;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][0] = s, red[threadIdx.x >> 6][1] = u;
+    __syncthreads();
+    const int k = threadIdx.x & (NW - 1);
+    SoftRow r = {m, red[k][0], red[k][1]};
+#pragma unroll
+    for (int o = NW / 2; o > 0; o >>= 1) {
+        r.s += __shfl_xor(r.s, o, 64);
+        if (ENT) r.u += __shfl_xor(r.u, o, 64);
+    }
+    return r;
+}
+// the statistics of a block's threads merged: the maximum first, then the
+// sums (each thread rescales its own once)
+template <int NW, bool ENT>
+__device__ __forceinline__ SoftRow soft_block(const Soft& st, float c2, float* redm,
+                                              double (*red)[2]) {
+    const float m = block_maxf<NW>(st.m, redm);
+    const float d = st.m - soft_ref(m), f = __builtin_amdgcn_exp2f(d * c2);
+    return block_sums<NW, ENT>(m, st.s * f, f * (st.u + st.s * fmaxf(d, kFar)), red);
+}
+
+// exp and log in 64 bits to about 1e-11 relative, for the one thread of a
+// block that finishes a row: Taylor's series after the usual reduction, a
+// handful of registers where the library's take some 60, which rows held in
+// registers do not have to spare (the policy kernel spilled 84 to 142 of 128
+// registers around them and ran twice as long).
+__device__ __forceinline__ double exp_small(double x) {  // |x| <= 0.35
+    double p = 1.0 / 3628800.0;
+    p = fma(p, x, 1.0 / 362880.0);
+    p = fma(p, x, 1.0 / 40320.0);
+    p = fma(p, x, 1.0 / 5040.0);
+    p = fma(p, x, 1.0 / 720.0);
+    p = fma(p, x, 1.0 / 120.0);
+    p = fma(p, x, 1.0 / 24.0);
+    p = fma(p, x, 1.0 / 6.0);
+    p = fma(p, x, 0.5);
+    p = fma(p, x, 1.0);
+    return fma(p, x, 1.0);
+}
+constexpr double kLn2 = 0.69314718055994530942;
+__device__ __forceinline__ double exp_d(double x) {  // |x| <= 700
+    const double n = rint(x * (1.0 / kLn2));
+    return ldexp(exp_small(fma(n, -kLn2, x)), (int)n);
+}
+// From log2 in F32, L: log S = L ln 2 + log(S 2^-L), the last term by its
+// series at a value within 2e-6 of 1.
+__device__ __forceinline__ double log_d(double S) {
+    const float L = __builtin_amdgcn_logf((float)S), n = rintf(L);
+    const double e = ldexp(exp_small((double)(n - L) * kLn2), -(int)n);
+    const double t = fma(S, e, -1.0);
+    return fma((double)L, kLn2, fma(-0.5 * t, t, t));
 }
 
 struct RowOut {
-    float logp, lse, ent;
+    double logp;
+    float lse, ent;
 };
-__device__ __forceinline__ RowOut row_out(const Soft& st, float ft, bool has_t, float c) {
-    const float ls = st.s > 0.f || st.s != st.s ? logf(st.s) : NAN;  // nothing above -Inf
+__device__ __forceinline__ RowOut row_out(const SoftRow& st, float ft, bool has_t, float c) {
+    // (nothing above -Inf: NaN)
+    const double ls = st.s > 0.0 || st.s != st.s ? log_d(st.s) : (double)NAN;
     RowOut o;
-    o.logp = has_t ? c * (ft - st.m) - ls : NAN;
-    o.lse = c * st.m + ls;
-    o.ent = ls - c * (st.u / st.s);
+    o.logp = has_t ? (double)c * ((double)ft - (double)st.m) - ls : (double)NAN;
+    o.lse = (float)((double)c * (double)st.m + ls);
+    o.ent = (float)(ls - (double)(c * ((float)st.u / (float)st.s)));
     return o;
 }
 

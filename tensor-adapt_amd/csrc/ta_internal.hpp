@@ -17,6 +17,8 @@
 namespace ta {
 
 void* scratch_get(size_t bytes, hipStream_t s, int slot = 0);
+// whether s records a graph (also where the runtime refuses to say)
+bool is_capturing(hipStream_t s);
 
 // Kernel ids of the kernel-level timer (ta_kprof_select).
 enum KernelId {

@@ -366,7 +366,7 @@ def test_preference_loss(kind, lens):
             tgt = tokens(g, n + 9, 50, 0.3)
             off = torch.tensor(np.cumsum([2] + lens), device=DEV, dtype=torch.int64)
             f32 = lambda v: float(np.float32(v))
-            par = (kind, average, f32(0.1), f32(0.1) if kind == 0 else 0.0, f32(0.05), f32(0.25))
+            par = (kind, average, f32(0.1), f32(0.1), f32(0.05), f32(0.25))
             check_pref(run_pref(logp, ref, tgt, off, *par), ref_pref(logp, ref, tgt, off, *par))
 
 
@@ -570,11 +570,19 @@ def test_policy_loss_logits(N, V):
         close(o[0], wl, ltol, "logp")
         if ec:
             close(o[1], we, 4 * (math.log(V) + 2) * sum_tol(V), "entropy")
-        # the loss and dlogp of the logp that came out
+        # the loss and dlogp of the logp that came out, up to its rounding: the
+        # kernel goes on with the logp before it is rounded to F32, which the
+        # result is within EPS |logp| of; d(loss) = |A| r + kl_beta |1 - e^d|
+        # and d(kl) = |1 - e^d| times that (r, e^d of the rounded logp, the
+        # second order and far ratios within the factor 1.01)
         want = ref_policy(o[0], i["old"], ref, i["adv"], w, f32(0.2), f32(0.3), 2.0, f32(0.04),
                           f32(ec), o[1].double() if ec else None)
-        close(o[2], want[0], 8 * EPS * (want[0].abs() + want[1].abs() + f32(ec) * 13) + 1e-30, "loss")
-        close(o[3], want[1], 8 * EPS * want[1].abs() + 1e-30, "kl")
+        off = EPS * o[0].double().abs() * 1.01
+        dkl = (ref.double() - o[0]).expm1().abs() if ref is not None else 0.0
+        dpg = i["adv"].double().abs() * (o[0].double() - i["old"]).exp()
+        close(o[2], want[0], 8 * EPS * (want[0].abs() + want[1].abs() + f32(ec) * 13)
+              + off * (dpg + f32(0.04) * dkl) + 1e-30, "loss")
+        close(o[3], want[1], 8 * EPS * want[1].abs() + off * dkl + 1e-30, "kl")
         # (loss and gradient of the same call cannot be told apart further)
         check_bwd(keep, torch.where(on, t, torch.full_like(t, -1)), f32(c), d, want[2].float(),
                   (-f32(ec) * w).float() if ec else None, V)

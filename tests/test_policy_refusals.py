@@ -51,7 +51,7 @@ CASES = [
     ("ta_preference_loss", PREF, [
         (dict(P=-1), "bad shape"), (dict(N=-1), "bad shape"), (dict(kind=3), "kind"),
         (dict(average=2), "average"), (dict(beta=F(0)), "beta"), (dict(beta=F(NAN)), "beta"),
-        (dict(smoothing=F(1)), "smoothing"), (dict(smoothing=F(0.1), kind=1), "sigmoid"),
+        (dict(smoothing=F(1)), "smoothing"), (dict(smoothing=F(-0.1), kind=1), "smoothing"),
         (dict(margin=F(INF)), "finite"), (dict(scale=F(NAN)), "finite"),
         (dict(offsets=None), "null"), (dict(logp=None), "null"), (dict(pair_loss=None), "null")]),
     ("ta_policy_loss", POL, [

@@ -131,6 +131,48 @@ int ta_engine_step(void* engine, const int32_t* inputs, const int32_t* targets,
 int ta_engine_step_resident(void* engine, const int32_t* d_inputs, const int32_t* d_targets,
                             float lr_override, ta_step_metrics* metrics);
 
+/* ── preference and policy fine-tuning ───────────────────────────────
+ * No counterpart in the reference, which trains on the cross entropy alone.
+ * Batches are host token ids [B*T] as in ta_engine_step, but the targets are
+ * taken as they are: a target < 0 (a prompt's or padding's) does not count, a
+ * target >= vocab is refused.  The token arrays are host F32 [B*T]; those the
+ * step makes stay readable as the buffers "logp", "entropy", "kl", "dlogp",
+ * "pair_loss", "rewards" (their memory is allocated at the first call of
+ * these three).
+ *
+ * ta_engine_logp: the log-probability of every counting target (0 for the
+ * others) and, unless NULL, the entropy of its distribution, with the adapter
+ * (use_adapter 1: the old log-probabilities of a policy step) or of the
+ * frozen base alone (0: the reference's).  The logits are rounded to BF16 as
+ * the steps' are, and not stored (ta_lm_head_logp).  No state changes. */
+int ta_engine_logp(void* engine, const int32_t* inputs, const int32_t* targets, int use_adapter,
+                   float* logp, float* entropy);
+
+/* One step on a preference loss (ta_preference_loss): rows 2p and 2p + 1 of
+ * the batch are the chosen and the rejected answer of pair p (B even), the
+ * loss is the mean over the pairs.  ref_logp (may be NULL: no reference) as
+ * ta_engine_logp(.., 0, ..) gave it.  Metrics as ta_engine_step's, loss the
+ * mean pair loss, valid_tokens the counting tokens, nonfinite_logits -1. */
+typedef struct ta_preference_config {
+    int kind; /* TA_PREF_SIGMOID, TA_PREF_IPO, TA_PREF_HINGE (ta_backend.h) */
+    int average;
+    float beta, smoothing, margin;
+} ta_preference_config;
+int ta_engine_step_preference(void* engine, const int32_t* inputs, const int32_t* targets,
+                              const float* ref_logp, const ta_preference_config* cfg,
+                              float lr_override, ta_step_metrics* metrics);
+
+/* One step on the clipped policy loss (ta_policy_loss_logits): loss = the sum
+ * of weight * token loss.  old_logp and ref_logp may be NULL as there.
+ * Metrics as above, valid_tokens the counting tokens of nonzero weight. */
+typedef struct ta_policy_config {
+    float clip_lo, clip_hi, dual_clip, kl_beta, ent_coef, inv_temp;
+} ta_policy_config;
+int ta_engine_step_policy(void* engine, const int32_t* inputs, const int32_t* targets,
+                          const float* old_logp, const float* ref_logp, const float* adv,
+                          const float* weight, const ta_policy_config* cfg, float lr_override,
+                          ta_step_metrics* metrics);
+
 /* Kernel-class timing during real steps.  category (TA_CAT_*) selects which
  * launches are bracketed with HIP events on the engine's stream (-1: none);
  * each step then adds their summed duration, launch count and algorithmic

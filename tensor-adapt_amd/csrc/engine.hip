@@ -59,6 +59,21 @@ struct Layer {
     float *in_rms, *post_rms, *attn_st, *ao32;  // attn_st: rows' (max, 1/sum); ao32: output in F32
 };
 
+// The loss of a step: the cross entropy (CE), or one of the preference and
+// policy losses, whose token arrays live in Policy.
+enum Objective { OBJ_CE = 0, OBJ_PREFERENCE, OBJ_POLICY };
+
+// Buffers of scoring and of the preference and policy steps, allocated at the
+// first of them (a handful of floats per token).
+struct Policy {
+    bool ready = false;
+    float *logp, *lse, *entropy, *dlogp, *kl;          // results per token
+    float *old_logp, *ref, *adv, *weight;              // inputs per token
+    float *pair_loss, *rewards;                        // [B / 2], [B]
+    int64_t* offsets;                                  // sequence q starts at q T
+    float* host = nullptr;                             // pinned staging, 4 BT + 2 B floats
+};
+
 struct Engine {
     ta_model_config mc;
     ta_adapt_config ac;
@@ -136,6 +151,12 @@ struct Engine {
     int64_t step_count = 0;
     float phase[3] = {0, 0, 0};
     const int32_t* tok_cur = nullptr;  // token ids the forward embeds
+    Objective obj = OBJ_CE;            // loss of the current step
+    ta_preference_config pref_cfg;
+    ta_policy_config pol_cfg;
+    bool has_old = false, has_ref = false;  // the step's old_logp / ref_logp
+    bool lora_off = false;                  // forward of the base alone (scoring)
+    Policy pol;
 
     // kernel-class timing (ta_engine_profile)
     int prof_cat = -1;
@@ -493,6 +514,7 @@ static inline double gbytes(double M, double N, double K, double in_b, double ou
 // the epilogue of y_p's projection GEMM (fwd_epi).
 static int lora_group_h(Engine* e, Layer& ly, std::initializer_list<int> group, const bf16* x,
                         int in) {
+    if (e->lora_off) return 0;
     const bf16* Ay[3];
     bf16* hs[3];
     int n = 0;
@@ -510,7 +532,7 @@ static int lora_group_h(Engine* e, Layer& ly, std::initializer_list<int> group, 
 
 static LoraEpi fwd_epi(Engine* e, const Pair& pr) {
     LoraEpi ep{};
-    if (!pr.on) return ep;
+    if (!pr.on || e->lora_off) return ep;
     ep.n = 1;
     ep.r = e->r;
     ep.delta = true;
@@ -731,7 +753,8 @@ static int layer_fwd_body(Engine* e, Layer& ly) {
     return 0;
 }
 
-static int forward(Engine* e) {
+// Embedding to final norm (qwen2.cu:47-161).
+static int forward_body(Engine* e) {
     const ta_model_config& c = e->mc;
     const int BT = e->BT, H = e->H, I = e->I;
     const double dBT = BT;
@@ -760,10 +783,49 @@ static int forward(Engine* e) {
                           last ? e->xfn : e->L[l + 1].xn, last ? e->final_rms : e->L[l + 1].in_rms,
                           BT, H, c.rms_eps, s));
     }
+    return 0;
+}
+
+// Preference or policy loss of the logits, whose gradient overwrites them.
+static int policy_objective(Engine* e) {
+    Policy& p = e->pol;
+    const int BT = e->BT, V = e->V;
+    const double dBT = BT;
+    hipStream_t s = e->s;
+    if (e->obj == OBJ_POLICY) {
+        const ta_policy_config& c = e->pol_cfg;
+        TIMED(TA_CAT_CE, 0, dBT * V * 4,
+              ta_policy_loss_logits(e->logits, V, e->tgt_dev, c.inv_temp,
+                                    e->has_old ? p.old_logp : nullptr,
+                                    e->has_ref ? p.ref : nullptr, p.adv, p.weight, c.clip_lo,
+                                    c.clip_hi, c.dual_clip, c.kl_beta, c.ent_coef, p.logp,
+                                    p.entropy, e->loss_tok, p.kl, e->logits, V, BT, V, s));
+        return 0;
+    }
+    const ta_preference_config& c = e->pref_cfg;
+    const int pairs = e->B / 2;
+    TIMED(TA_CAT_CE, 0, dBT * V * 2,
+          ta_token_logp_fwd(e->logits, V, e->tgt_dev, 1.f, p.logp, p.lse, nullptr, BT, V, s));
+    TIMED(TA_CAT_CE, 0, dBT * 16,
+          ta_preference_loss(p.logp, e->has_ref ? p.ref : nullptr, e->tgt_dev, p.offsets, pairs, BT,
+                             c.kind, c.average, c.beta, c.smoothing, c.margin, 1.f / (float)pairs,
+                             p.pair_loss, p.rewards, p.dlogp, s));
+    TIMED(TA_CAT_CE, 0, dBT * V * 4,
+          ta_token_logp_bwd(e->logits, V, e->tgt_dev, 1.f, p.lse, nullptr, p.dlogp, nullptr,
+                            e->logits, V, BT, V, s));
+    return 0;
+}
+
+static int forward(Engine* e) {
+    const int BT = e->BT, H = e->H;
+    const double dBT = BT;
+    hipStream_t s = e->s;
+    CK(forward_body(e));
     // LM head (qwen2.cu:163-175), tied to the embedding when c.tie
     TIMED(TA_CAT_LMHEAD, gflops(BT, e->V, H), gbytes(BT, e->V, H, 2, 2, false),
           gemm_dispatch(true, true, BT, e->V, H, 1.f, e->xfn, H, e->lm, H, 0.f, e->logits, e->V,
                         nullptr, s, 0, nullptr));
+    if (e->obj != OBJ_CE) return policy_objective(e);
     // loss (adapt_trainer.cu:201-205): dlogits overwrite the logits in place
     // (one read and one write of BT x V BF16); the first step also counts
     // the NaN and Inf logits (adapt_trainer.cu:196-198)
@@ -786,7 +848,7 @@ static int backward(Engine* e) {
     const double nrm_b = dBT * H * 6 + H * 2 + dBT * 4;
     e->wg_cursor = 0;
     // dres = dlogits * W_lm (qwen2.cu:205); grad = rms_norm_bwd(final)
-    if (e->ce_in_dx)
+    if (e->ce_in_dx && e->obj == OBJ_CE)
         TIMED(TA_CAT_LMHEAD_BWD, gflops(BT, H, e->V), gbytes(BT, H, e->V, 2, 2, false),
               gemm_ce_dx(BT, H, e->V, e->logits, e->lmT, e->dres, e->lse2, e->tgt_dev,
                          1.f / (float)BT, s));
@@ -909,7 +971,11 @@ static int engine_step_body(Engine* e, float lr_override, ta_step_metrics* m,
     CK(backward(e));
     TA_HIP(hipEventRecord(e->ev[2], e->s));
     // tail: loss read-back, grad norm + clip + AdamW on the device
-    TA_HIP(hipMemcpyAsync(e->loss_host, e->loss_tok, BT * 4, hipMemcpyDeviceToHost, e->s));
+    if (e->obj == OBJ_PREFERENCE)
+        TA_HIP(hipMemcpyAsync(e->pol.host + 4 * (int64_t)BT, e->pol.pair_loss, (e->B / 2) * 4,
+                              hipMemcpyDeviceToHost, e->s));
+    else
+        TA_HIP(hipMemcpyAsync(e->loss_host, e->loss_tok, BT * 4, hipMemcpyDeviceToHost, e->s));
     float lr = (lr_override > 0.f)
                    ? lr_override
                    : cosine_lr(e->ac.lr, e->ac.warmup, e->ac.total_steps, 0.1f, e->step_count);
@@ -925,15 +991,31 @@ static int engine_step_body(Engine* e, float lr_override, ta_step_metrics* m,
     TA_HIP(hipStreamSynchronize(e->s));
     for (int i = 0; i < 3; i++) TA_HIP(hipEventElapsedTime(&e->phase[i], e->ev[i], e->ev[i + 1]));
     CK(prof_collect(e));
-    // adapt_trainer.cu:237-246: mean over tokens whose loss > 1e-9
     float mean = 0.f;
     int valid = 0;
-    for (int i = 0; i < BT; i++)
-        if (e->loss_host[i] > 1e-9f) {
-            mean += e->loss_host[i];
-            valid++;
+    if (e->obj == OBJ_CE) {
+        // adapt_trainer.cu:237-246: mean over tokens whose loss > 1e-9
+        for (int i = 0; i < BT; i++)
+            if (e->loss_host[i] > 1e-9f) {
+                mean += e->loss_host[i];
+                valid++;
+            }
+        if (valid > 0) mean /= (float)valid;
+    } else {
+        // the mean of the pairs, or the weighted sum of the tokens
+        const float* w = e->pol.host + 3 * (int64_t)BT;
+        const float* pairs = e->pol.host + 4 * (int64_t)BT;
+        const bool pol = e->obj == OBJ_POLICY;
+        double sum = 0.0;
+        for (int i = 0; i < BT; i++) {
+            const bool on = e->tgt_host[i] >= 0 && (!pol || w[i] != 0.f);
+            valid += on;
+            if (pol && on) sum += (double)w[i] * (double)e->loss_host[i];
         }
-    if (valid > 0) mean /= (float)valid;
+        if (!pol)
+            for (int i = 0; i < e->B / 2; i++) sum += (double)pairs[i] / (e->B / 2);
+        mean = (float)sum;
+    }
     float norm = e->norm_host[0];
     int32_t bad, nonfinite;
     memcpy(&bad, e->norm_host + 1, sizeof bad);
@@ -952,7 +1034,7 @@ static int engine_step_body(Engine* e, float lr_override, ta_step_metrics* m,
         m->gnorm = std::min(norm, e->ac.grad_clip);
         m->valid_tokens = valid;
         m->step = (int)e->step_count;
-        m->nonfinite_logits = first ? nonfinite : -1;
+        m->nonfinite_logits = first && e->obj == OBJ_CE ? nonfinite : -1;
         m->step_ms =
             std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now() - t0).count();
     }
@@ -970,6 +1052,88 @@ static int engine_step(Engine* e, const int32_t* inputs, const int32_t* targets,
     TA_HIP(hipMemcpyAsync(e->tgt_dev, e->tgt_host, BT * 4, hipMemcpyHostToDevice, e->s));
     e->tok_cur = e->tok_dev;
     return engine_step_body(e, lr_override, m, t0);
+}
+
+// ── preference and policy steps ─────────────────────────────────────────
+static int policy_alloc(Engine* e) {
+    Policy& p = e->pol;
+    if (p.ready) return 0;
+    const int64_t BT = e->BT, B = e->B;
+    CK(alloc(e, &p.logp, BT, "logp", 1));
+    CK(alloc(e, &p.lse, BT, "lse", 1));
+    CK(alloc(e, &p.entropy, BT, "entropy", 1));
+    CK(alloc(e, &p.dlogp, BT, "dlogp", 1));
+    CK(alloc(e, &p.kl, BT, "kl", 1));
+    CK(alloc(e, &p.old_logp, BT, "policy.old"));
+    CK(alloc(e, &p.ref, BT, "policy.ref"));
+    CK(alloc(e, &p.adv, BT, "policy.adv"));
+    CK(alloc(e, &p.weight, BT, "policy.weight"));
+    CK(alloc(e, &p.pair_loss, (B + 1) / 2, "pair_loss", 1));
+    CK(alloc(e, &p.rewards, B, "rewards", 1));
+    CK(alloc(e, &p.offsets, B + 1, "policy.offsets"));
+    if (!p.host) TA_HIP(hipHostMalloc((void**)&p.host, (4 * BT + 2 * B) * sizeof(float)));
+    std::vector<int64_t> off(B + 1);
+    for (int64_t q = 0; q <= B; q++) off[q] = q * e->T;
+    TA_HIP(hipMemcpyAsync(p.offsets, off.data(), off.size() * sizeof(int64_t),
+                          hipMemcpyHostToDevice, e->s));
+    TA_HIP(hipStreamSynchronize(e->s));
+    p.ready = true;
+    return 0;
+}
+// The batch as given (targets < 0: not counted; no assistant-span masking).
+static int policy_batch(Engine* e, const char* what, const int32_t* inputs,
+                        const int32_t* targets) {
+    for (int i = 0; i < e->BT; i++) {
+        TA_REQUIRE(inputs[i] >= 0 && inputs[i] < e->V, "%s: token id %d out of range", what,
+                   inputs[i]);
+        TA_REQUIRE(targets[i] < e->V, "%s: target id %d out of range", what, targets[i]);
+    }
+    CK(policy_alloc(e));
+    const size_t n = (size_t)e->BT * sizeof(int32_t);
+    memcpy(e->tok_host, inputs, n);
+    memcpy(e->tgt_host, targets, n);
+    TA_HIP(hipMemcpyAsync(e->tok_dev, e->tok_host, n, hipMemcpyHostToDevice, e->s));
+    TA_HIP(hipMemcpyAsync(e->tgt_dev, e->tgt_host, n, hipMemcpyHostToDevice, e->s));
+    e->tok_cur = e->tok_dev;
+    return 0;
+}
+// token array `slot` of the staging block to dst
+static int policy_upload(Engine* e, int slot, const float* src, float* dst) {
+    float* h = e->pol.host + (int64_t)slot * e->BT;
+    memcpy(h, src, (size_t)e->BT * sizeof(float));
+    TA_HIP(hipMemcpyAsync(dst, h, (size_t)e->BT * sizeof(float), hipMemcpyHostToDevice, e->s));
+    return 0;
+}
+static int policy_step(Engine* e, Objective obj, float lr_override, ta_step_metrics* m,
+                       std::chrono::steady_clock::time_point t0) {
+    e->obj = obj;
+    const int rc = engine_step_body(e, lr_override, m, t0);
+    e->obj = OBJ_CE;
+    return rc;
+}
+
+static int engine_logp(Engine* e, bool use_adapter, float* logp, float* entropy) {
+    Policy& p = e->pol;
+    TA_HIP(hipMemsetAsync(e->bad_dev, 0, sizeof(int32_t), e->s));
+    e->lora_off = !use_adapter;
+    int rc = forward_body(e);
+    e->lora_off = false;
+    CK(rc);
+    // (the logits' buffer is the workspace: it has 2 V bytes a row, the
+    // partial statistics take 3 floats per 128 columns and one more)
+    static_assert(sizeof(bf16) == 2, "");
+    void* ws = ta_lm_head_logp_ws(e->BT, e->V) <= (int64_t)e->BT * e->V * 2 ? e->logits : nullptr;
+    TIMED(TA_CAT_LMHEAD, gflops(e->BT, e->V, e->H), gbytes(e->BT, e->V, e->H, 2, 0, false),
+          ta_lm_head_logp(e->xfn, e->H, e->lm, e->H, e->tgt_dev, 1.f, 1, p.logp, p.lse, p.entropy,
+                          e->BT, e->V, e->H, ws, e->s));
+    const size_t n = (size_t)e->BT * sizeof(float);
+    TA_HIP(hipMemcpyAsync(p.host, p.logp, n, hipMemcpyDeviceToHost, e->s));
+    TA_HIP(hipMemcpyAsync(p.host + e->BT, p.entropy, n, hipMemcpyDeviceToHost, e->s));
+    TA_HIP(hipStreamSynchronize(e->s));
+    CK(prof_collect(e));
+    memcpy(logp, p.host, n);
+    if (entropy) memcpy(entropy, p.host + e->BT, n);
+    return 0;
 }
 
 static bf16** weight_slot(Engine* e, const std::string& name, int64_t* n, int* layer, int* proj) {
@@ -1109,7 +1273,7 @@ int ta_engine_destroy(void* ep) {
     if (e->s) (void)hipStreamSynchronize(e->s);
     for (void* p : e->allocs) (void)hipFree(p);
     for (void* p : {(void*)e->tok_host, (void*)e->tgt_host, (void*)e->loss_host,
-                    (void*)e->norm_host})
+                    (void*)e->norm_host, (void*)e->pol.host})
         if (p) (void)hipHostFree(p);
     for (auto& ev : e->ev)
         if (ev) (void)hipEventDestroy(ev);
@@ -1267,6 +1431,53 @@ int ta_engine_step_resident(void* ep, const int32_t* d_inputs, const int32_t* d_
     CK(mask_targets_dev(d_inputs, d_targets, e->tgt_dev, e->B, e->T, e->s));
     e->tok_cur = d_inputs;
     return engine_step_body(e, lr_override, m, t0);
+}
+
+int ta_engine_logp(void* ep, const int32_t* inputs, const int32_t* targets, int use_adapter,
+                   float* logp, float* entropy) {
+    Engine* e = (Engine*)ep;
+    TA_REQUIRE(e && inputs && targets && logp, "engine_logp: null argument");
+    TA_REQUIRE(use_adapter == 0 || use_adapter == 1, "engine_logp: use_adapter must be 0 or 1");
+    CK(policy_batch(e, "engine_logp", inputs, targets));
+    return engine_logp(e, use_adapter != 0, logp, entropy);
+}
+
+int ta_engine_step_preference(void* ep, const int32_t* inputs, const int32_t* targets,
+                              const float* ref_logp, const ta_preference_config* cfg,
+                              float lr_override, ta_step_metrics* m) {
+    Engine* e = (Engine*)ep;
+    TA_REQUIRE(e && inputs && targets && cfg, "engine_step_preference: null argument");
+    TA_REQUIRE(e->B % 2 == 0, "engine_step_preference: B = %d is not a number of pairs", e->B);
+    // (what the loss itself would refuse in the middle of the step)
+    CK(ta_preference_loss(nullptr, nullptr, nullptr, nullptr, 0, 0, cfg->kind, cfg->average,
+                          cfg->beta, cfg->smoothing, cfg->margin, 1.f, nullptr, nullptr, nullptr,
+                          nullptr));
+    auto t0 = std::chrono::steady_clock::now();
+    CK(policy_batch(e, "engine_step_preference", inputs, targets));
+    e->pref_cfg = *cfg;
+    e->has_ref = ref_logp != nullptr;
+    if (ref_logp) CK(policy_upload(e, 0, ref_logp, e->pol.ref));
+    return policy_step(e, OBJ_PREFERENCE, lr_override, m, t0);
+}
+
+int ta_engine_step_policy(void* ep, const int32_t* inputs, const int32_t* targets,
+                          const float* old_logp, const float* ref_logp, const float* adv,
+                          const float* weight, const ta_policy_config* cfg, float lr_override,
+                          ta_step_metrics* m) {
+    Engine* e = (Engine*)ep;
+    TA_REQUIRE(e && inputs && targets && adv && weight && cfg, "engine_step_policy: null argument");
+    CK(policy_config_check("engine_step_policy", cfg->clip_lo, cfg->clip_hi, cfg->dual_clip,
+                           cfg->kl_beta, cfg->ent_coef, cfg->inv_temp));
+    auto t0 = std::chrono::steady_clock::now();
+    CK(policy_batch(e, "engine_step_policy", inputs, targets));
+    e->pol_cfg = *cfg;
+    e->has_old = old_logp != nullptr;
+    e->has_ref = ref_logp != nullptr;
+    if (old_logp) CK(policy_upload(e, 0, old_logp, e->pol.old_logp));
+    if (ref_logp) CK(policy_upload(e, 1, ref_logp, e->pol.ref));
+    CK(policy_upload(e, 2, adv, e->pol.adv));
+    CK(policy_upload(e, 3, weight, e->pol.weight));
+    return policy_step(e, OBJ_POLICY, lr_override, m, t0);
 }
 
 int ta_engine_profile(void* ep, int category) {

@@ -739,9 +739,9 @@ static int token_logp_bwd(const T* logits, int64_t ld, const int32_t* targets, f
     return check_launch("token_logp_bwd");
 }
 
-static int policy_args(const char* what, const float* adv, const float* weight, float lo, float hi,
-                       float dual, float kl_beta, float ent_coef) {
-    TA_REQUIRE(adv && weight, "%s: null argument", what);
+int policy_config_check(const char* what, float lo, float hi, float dual, float kl_beta,
+                        float ent_coef, float inv_temp) {
+    TA_REQUIRE(temp_ok(inv_temp), "%s: inv_temp must be positive and finite", what);
     TA_REQUIRE(lo >= 0.f && lo < 1.f && hi >= 0.f && hi < INFINITY,
                "%s: clip range 1 - %g .. 1 + %g", what, lo, hi);
     TA_REQUIRE(dual == 0.f || (dual > 1.f && dual < INFINITY),
@@ -814,8 +814,8 @@ int ta_policy_loss(const float* logp, const float* old_logp, const float* ref_lo
                    int64_t N, void* stream) {
     TA_REQUIRE(N >= 0, "policy_loss: bad shape N=%lld", (long long)N);
     if (N == 0) return 0;
-    TA_REQUIRE(logp && dlogp, "policy_loss: null argument");
-    if (int rc = policy_args("policy_loss", adv, weight, clip_lo, clip_hi, dual_clip, kl_beta, 0.f))
+    TA_REQUIRE(logp && adv && weight && dlogp, "policy_loss: null argument");
+    if (int rc = policy_config_check("policy_loss", clip_lo, clip_hi, dual_clip, kl_beta, 0.f, 1.f))
         return rc;
     const PolicyArgs a{old_logp, ref_logp, adv, weight, clip_lo, clip_hi, dual_clip, kl_beta, 0.f};
     const int64_t blocks = (N + 255) / 256;
@@ -833,12 +833,12 @@ int ta_policy_loss_logits(const uint16_t* logits, int64_t ld, const int32_t* tar
     TA_REQUIRE(N >= 0 && V > 0 && ld >= V && ldd >= V,
                "policy_loss_logits: bad shape N=%d V=%d ld=%lld ldd=%lld", N, V, (long long)ld,
                (long long)ldd);
-    TA_REQUIRE(temp_ok(inv_temp), "policy_loss_logits: inv_temp must be positive and finite");
-    if (N == 0) return 0;
-    TA_REQUIRE(logits && targets && logp && loss && dlogits, "policy_loss_logits: null argument");
-    if (int rc = policy_args("policy_loss_logits", adv, weight, clip_lo, clip_hi, dual_clip,
-                             kl_beta, ent_coef))
+    if (int rc = policy_config_check("policy_loss_logits", clip_lo, clip_hi, dual_clip, kl_beta,
+                                     ent_coef, inv_temp))
         return rc;
+    if (N == 0) return 0;
+    TA_REQUIRE(logits && targets && adv && weight && logp && loss && dlogits,
+               "policy_loss_logits: null argument");
     TA_REQUIRE(ent_coef == 0.f || entropy, "policy_loss_logits: ent_coef needs the entropy");
     TA_REQUIRE((((uintptr_t)logits | (uintptr_t)dlogits) & 1) == 0,
                "policy_loss_logits: misaligned rows");

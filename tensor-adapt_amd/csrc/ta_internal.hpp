@@ -212,6 +212,9 @@ bool cross_entropy_lse_ok(const bf16* logits, int V);
 // Y = W^T [N x K], C = dX [M x N], all K-contiguous, beta 0).
 int gemm_ce_dx(int M, int N, int K, const bf16* logits, const bf16* Wt, bf16* C,
                const float* lse2, const int32_t* tgt, float inv_n, hipStream_t s);
+// whether the parameters of a policy loss are in range (else the error is set)
+int policy_config_check(const char* what, float clip_lo, float clip_hi, float dual_clip,
+                        float kl_beta, float ent_coef, float inv_temp);
 int fill_normal_bf16(bf16* out, int64_t n, uint64_t seed, uint64_t sid, float std, hipStream_t s);
 int fill_bf16(bf16* out, int64_t n, float v, hipStream_t s);
 int kaiming_init(float* a32, bf16* a16, int64_t n, int in_dim, hipStream_t s);

@@ -161,6 +161,18 @@ class StepMetrics(ctypes.Structure):
                 ("nonfinite_logits", ctypes.c_int)]
 
 
+class PreferenceConfig(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int), ("average", ctypes.c_int), ("beta", ctypes.c_float),
+                ("smoothing", ctypes.c_float), ("margin", ctypes.c_float)]
+
+
+class PolicyConfig(ctypes.Structure):
+    _fields_ = [("clip_lo", ctypes.c_float), ("clip_hi", ctypes.c_float),
+                ("dual_clip", ctypes.c_float), ("kl_beta", ctypes.c_float),
+                ("ent_coef", ctypes.c_float), ("inv_temp", ctypes.c_float)]
+
+
+PREFERENCE_LOSSES = {"sigmoid": 0, "ipo": 1, "hinge": 2}
 TARGETS = ("q", "k", "v", "o", "gate", "up", "down")
 WHICH = {"A": 0, "B": 1, "mA": 2, "vA": 3, "mB": 4, "vB": 5, "gA": 6, "gB": 7,
          "A16": 8, "B16": 9}
@@ -214,6 +226,51 @@ class Engine:
         m = StepMetrics()
         call("ta_engine_step_resident", self.h, ptr(d_inputs), ptr(d_targets), lr_override,
              ctypes.byref(m))
+        return {k: getattr(m, k) for k, _ in StepMetrics._fields_}
+
+    def _batch(self, *arrays):
+        """Host arrays of one value per token (None stays None): int32 ids,
+        then F32 values; kept alive by the caller."""
+        import numpy as np
+        out = []
+        for k, a in enumerate(arrays):
+            if a is not None:
+                a = np.ascontiguousarray(a, np.int32 if k < 2 else np.float32).reshape(-1)
+                if a.size != self.B * self.T:
+                    raise BackendError(f"{a.size} values for {self.B * self.T} tokens")
+            out.append(a)
+        return out
+
+    def logp(self, inputs, targets, use_adapter=True, entropy=False):
+        """log-probability of every target >= 0 (else 0); with the entropy on request."""
+        import numpy as np
+        i, t = self._batch(inputs, targets)
+        out = np.empty(self.B * self.T, np.float32)
+        ent = np.empty_like(out) if entropy else None
+        call("ta_engine_logp", self.h, i.ctypes.data, t.ctypes.data, 1 if use_adapter else 0,
+             out.ctypes.data, ent.ctypes.data if entropy else None)
+        return (out, ent) if entropy else out
+
+    def step_preference(self, inputs, targets, ref_logp=None, loss="sigmoid", average=False,
+                        beta=0.1, smoothing=0.0, margin=0.0, lr_override=0.0):
+        i, t, r = self._batch(inputs, targets, ref_logp)
+        cfg = PreferenceConfig(PREFERENCE_LOSSES[loss], 1 if average else 0, beta, smoothing,
+                               margin)
+        m = StepMetrics()
+        call("ta_engine_step_preference", self.h, i.ctypes.data, t.ctypes.data,
+             None if r is None else r.ctypes.data, ctypes.byref(cfg), lr_override,
+             ctypes.byref(m))
+        return {k: getattr(m, k) for k, _ in StepMetrics._fields_}
+
+    def step_policy(self, inputs, targets, adv, weight, old_logp=None, ref_logp=None, clip_lo=0.2,
+                    clip_hi=0.2, dual_clip=0.0, kl_beta=0.0, ent_coef=0.0, inv_temp=1.0,
+                    lr_override=0.0):
+        i, t, a, w, o, r = self._batch(inputs, targets, adv, weight, old_logp, ref_logp)
+        cfg = PolicyConfig(clip_lo, clip_hi, dual_clip, kl_beta, ent_coef, inv_temp)
+        m = StepMetrics()
+        call("ta_engine_step_policy", self.h, i.ctypes.data, t.ctypes.data,
+             None if o is None else o.ctypes.data, None if r is None else r.ctypes.data,
+             a.ctypes.data, w.ctypes.data, ctypes.byref(cfg), lr_override, ctypes.byref(m))
         return {k: getattr(m, k) for k, _ in StepMetrics._fields_}
 
     def profile(self, category):

@@ -103,7 +103,11 @@ int ta_cross_entropy_fwd(const uint16_t* logits, const int32_t* targets, float* 
  * logits: rows of V values, ld elements apart (ld >= V), at any alignment of
  * their type.  A row with t < 0 has no token: its logits are not read and its
  * three results are 0.  A row with t >= V, a NaN, a +Inf or nothing above
- * -Inf gives NaN; single logits of -Inf have p = 0.  All sums are F32. */
+ * -Inf gives NaN; single logits of -Inf have p = 0.  V up to 2^30.  Terms are
+ * F32 and added in F32 by each thread, in 64 bits after that.  A few long rows
+ * (at most 512 of 192 KB or more) are split over blocks through the stream's
+ * scratch pool, in a captured call not: its sums then run in another order
+ * than the eager call's. */
 int ta_token_logp_fwd(const uint16_t* logits, int64_t ld, const int32_t* targets, float inv_temp,
                       float* logp, float* lse, float* entropy, int N, int V, void* stream);
 int ta_token_logp_fwd_f32(const float* logits, int64_t ld, const int32_t* targets, float inv_temp,
@@ -132,8 +136,9 @@ int ta_token_logp_bwd_f32(const float* logits, int64_t ld, const int32_t* target
  * 1 rounds each logit to BF16 first, as ta_gemm_bf16 writes it, so the result
  * is that of ta_token_logp_fwd on those logits up to the order of sums; 0
  * keeps them in F32.  ws: ta_lm_head_logp_ws(N, V) bytes of the caller's for
- * this call alone, or NULL: the stream's scratch pool.  Rows without a token
- * give 0 (their logits are still computed).  No reference counterpart. */
+ * this call alone (16-byte aligned), or NULL: the stream's scratch pool, not
+ * in a captured call.  Rows without a token give 0 (their logits are still
+ * computed).  V up to 2^30, N up to 2^25.  No reference counterpart. */
 int ta_lm_head_logp(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t ldw,
                     const int32_t* targets, float inv_temp, int round_logits, float* logp,
                     float* lse, float* entropy, int N, int V, int H, void* ws, void* stream);
@@ -187,7 +192,7 @@ int ta_policy_loss(const float* logp, const float* old_logp, const float* ref_lo
  * terms.  Rows without a token (t < 0 or weight 0) are not read; their
  * results and gradient are 0.  logp, entropy (may be NULL when ent_coef is 0)
  * and kl (may be NULL) get the row's values; dlogits may be logits itself
- * (with ldd = ld). */
+ * (with ldd = ld).  Splits few long rows as ta_token_logp_fwd does. */
 int ta_policy_loss_logits(const uint16_t* logits, int64_t ld, const int32_t* targets,
                           float inv_temp, const float* old_logp, const float* ref_logp,
                           const float* adv, const float* weight, float clip_lo, float clip_hi,

@@ -573,6 +573,10 @@ __device__ __forceinline__ double pref_pair(const PrefArgs& a, const PrefSums& q
     const double u = (pi[0] - rf[0]) - (pi[1] - rf[1]), beta = a.beta;
     const double z = beta * u - (double)a.margin, sm = a.smoothing;
     double du;
+    if (u != u) {  // (the maxima and tests below drop a NaN)
+        *loss = u;
+        return u;
+    }
     if (a.kind == TA_PREF_SIGMOID) {
         *loss = (1.0 - sm) * softplus(-z) + sm * softplus(z);
         // sigma(z) - (1 - smoothing), without cancelling at large z
@@ -583,8 +587,8 @@ __device__ __forceinline__ double pref_pair(const PrefArgs& a, const PrefSums& q
         *loss = v * v;
         du = 2.0 * v;
     } else {
-        *loss = z < 1.0 ? 1.0 - z : z - z;  // (NaN stays)
-        du = z < 1.0 ? -beta : z - z;
+        *loss = fmax(1.0 - z, 0.0);
+        du = z < 1.0 ? -beta : 0.0;
     }
     return du * (double)a.scale;
 }
@@ -648,6 +652,7 @@ __global__ __launch_bounds__(64 * NW) void k_preference(PrefArgs a) {
 
 // at most this many blocks of a launch over rows (its threads stay below 2^32)
 static inline dim3 row_grid(int64_t rows) { return dim3((unsigned)(rows < (1 << 20) ? rows : 1 << 20)); }
+constexpr int kMaxV = 1 << 30;  // indices into a row stay below 2^31
 static bool temp_ok(float c) { return c > 0.f && c < INFINITY; }
 
 // Whether rows take a block of two waves instead of eight: where eight have
@@ -677,7 +682,7 @@ static int grad_splits(int N, int V, int es) {
 template <typename T>
 static int token_logp_fwd(const T* logits, int64_t ld, const int32_t* targets, float c, float* logp,
                           float* lse, float* entropy, int N, int V, hipStream_t s) {
-    TA_REQUIRE(N >= 0 && V > 0 && ld >= V, "token_logp_fwd: bad shape N=%d V=%d ld=%lld", N, V,
+    TA_REQUIRE(N >= 0 && V > 0 && V <= kMaxV && ld >= V, "token_logp_fwd: bad shape N=%d V=%d ld=%lld", N, V,
                (long long)ld);
     TA_REQUIRE(temp_ok(c), "token_logp_fwd: inv_temp must be positive and finite");
     if (N == 0) return 0;
@@ -685,8 +690,9 @@ static int token_logp_fwd(const T* logits, int64_t ld, const int32_t* targets, f
     TA_REQUIRE(((uintptr_t)logits % sizeof(T)) == 0, "token_logp_fwd: misaligned logits");
     const int splits = row_splits(N, V, sizeof(T), 512, s);
     if (splits > 1) {
-        SoftRow* part = (SoftRow*)scratch_get(sizeof(SoftRow) * N * splits, s);
-        if (!part) return set_error(-2, "token_logp_fwd: scratch allocation failed");
+        SoftRow* part = nullptr;
+        if (int rc = scratch_here("token_logp_fwd", sizeof(SoftRow) * N * splits, s, (void**)&part))
+            return rc;
         const dim3 grid(N * splits);
         const float* no_weight = nullptr;
         if (entropy) {
@@ -722,7 +728,7 @@ static int token_logp_bwd(const T* logits, int64_t ld, const int32_t* targets, f
                           const float* lse, const float* entropy, const float* dlogp,
                           const float* dentropy, T* dlogits, int64_t ldd, int N, int V,
                           hipStream_t s) {
-    TA_REQUIRE(N >= 0 && V > 0 && ld >= V && ldd >= V,
+    TA_REQUIRE(N >= 0 && V > 0 && V <= kMaxV && ld >= V && ldd >= V,
                "token_logp_bwd: bad shape N=%d V=%d ld=%lld ldd=%lld", N, V, (long long)ld,
                (long long)ldd);
     TA_REQUIRE(temp_ok(c), "token_logp_bwd: inv_temp must be positive and finite");
@@ -830,7 +836,7 @@ int ta_policy_loss_logits(const uint16_t* logits, int64_t ld, const int32_t* tar
                           float dual_clip, float kl_beta, float ent_coef, float* logp,
                           float* entropy, float* loss, float* kl, uint16_t* dlogits, int64_t ldd,
                           int N, int V, void* stream) {
-    TA_REQUIRE(N >= 0 && V > 0 && ld >= V && ldd >= V,
+    TA_REQUIRE(N >= 0 && V > 0 && V <= kMaxV && ld >= V && ldd >= V,
                "policy_loss_logits: bad shape N=%d V=%d ld=%lld ldd=%lld", N, V, (long long)ld,
                (long long)ldd);
     if (int rc = policy_config_check("policy_loss_logits", clip_lo, clip_hi, dual_clip, kl_beta,
@@ -854,8 +860,10 @@ int ta_policy_loss_logits(const uint16_t* logits, int64_t ld, const int32_t* tar
     const int splits = row_splits(N, V, 2, 96, s);
     if (splits > 1) {
         const size_t gb = ((size_t)N * sizeof(GradRow) + 255) & ~(size_t)255;
-        char* ws = (char*)scratch_get(gb + sizeof(SoftRow) * N * splits, s);
-        if (!ws) return set_error(-2, "policy_loss_logits: scratch allocation failed");
+        char* ws = nullptr;
+        if (int rc = scratch_here("policy_loss_logits", gb + sizeof(SoftRow) * N * splits, s,
+                                  (void**)&ws))
+            return rc;
         GradRow* grads = (GradRow*)ws;
         SoftRow* part = (SoftRow*)(ws + gb);
         const dim3 grid(N * splits);

@@ -77,6 +77,19 @@ void* scratch_get(size_t bytes, hipStream_t s, int slot) {
     return sc.ptr;
 }
 
+int scratch_here(const char* what, size_t bytes, hipStream_t s, void** p) {
+    int dev = 0, own = 0;
+    TA_HIP(hipGetDevice(&dev));
+    if (s) {
+        TA_HIP(hipStreamGetDevice(s, &own));
+        TA_REQUIRE(own == dev, "%s: the stream is of device %d, the current one is %d", what, own,
+                   dev);
+    }
+    *p = scratch_get(bytes, s);
+    if (!*p) return set_error(-2, "%s: scratch allocation of %zu bytes failed", what, bytes);
+    return 0;
+}
+
 // Caching allocator behind the host API's Tensor (ta_mem_alloc/free).
 // Sizes round up to a power of two below 2 MiB and to a multiple of 2 MiB
 // above; a freed block goes back to its device's bin and is handed out again

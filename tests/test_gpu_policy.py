@@ -401,6 +401,10 @@ def test_preference_extremes_and_optional_outputs():
     logp = torch.tensor([0.0, -5e4, -5e4, 0.0], device=DEV)
     loss, _, d = run_pref(logp, None, tgt, off, 0, 0, 1.0, 0.0, 0.0, 1.0)
     assert loss.tolist() == [0.0, 5e4] and d.tolist() == [0.0, 0.0, -1.0, 1.0]
+    for kind in (0, 1, 2):
+        logp[0] = NAN
+        loss, rew, d = run_pref(logp, None, tgt, off, kind, 0, 1.0, 0.0, 0.0, 1.0)
+        assert np.isnan(loss[0]) and np.isnan(d[:2]).all() and np.isfinite(loss[1])
     for v in (NAN, INF):
         logp[0] = v
         loss, rew, d = run_pref(logp, None, tgt, off, 1, 0, 1.0, 0.0, 0.0, 1.0)
@@ -675,11 +679,20 @@ def test_lm_head_logp_captured_twice():
     ws = [torch.empty(need, device=DEV, dtype=torch.uint8) for _ in range(2)]
     outs = [[full(N) for _ in range(3)] for _ in range(2)]
     graphs = []
-    cap = torch.cuda.Stream()
-    torch.cuda.synchronize()
 
     def run(k, o, w):
         call("ta_lm_head_logp", P(hs[k]), H, P(W), H, P(t), F(1), 0, *map(P, o), N, V, H, P(w), S())
+    cap = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    refused = []
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=cap):
+        try:
+            run(0, outs[0], None)  # the pool's buffer is not for graphs
+        except tadapt.BackendError as e:
+            refused.append(str(e))
+        outs[0][0].fill_(1.0)
+    assert refused and "workspace" in refused[0]
     for k in range(2):
         gr = torch.cuda.CUDAGraph()
         with torch.cuda.graph(gr, stream=cap):
@@ -701,3 +714,46 @@ def test_lm_head_logp_captured_twice():
         for k in range(2):
             for a, b in zip(outs[k], want[k]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("N,V", [(3, 151936), (40, 110003)])
+def test_long_rows_captured_and_eager(N, V):
+    """A few long rows: eager calls split them over blocks, captured ones do
+    not, so the two agree to the sums' rounding; every replay gives the same
+    bits, also of another stream's graph at the same time."""
+    g = gen(V)
+    x, t = rows(g, N, V, BF16), tokens(g, N, V, 0.0)
+    i = policy_inputs(g, N, full(N, -8.0))
+
+    def run(o, d):
+        call("ta_token_logp_fwd", P(x), V, P(t), F(1), *map(P, o[:3]), N, V, S())
+        call("ta_policy_loss_logits", P(x), V, P(t), F(1), P(i["old"]), P(i["ref"]), P(i["adv"]),
+             P(i["weight"]), F(0.2), F(0.3), F(0), F(0.04), F(0.01), *map(P, o[3:]), P(d), V, N, V,
+             S())
+    outs = [[full(N) for _ in range(7)] for _ in range(3)]
+    ds = [torch.empty_like(x) for _ in range(3)]
+    run(outs[0], ds[0])
+    check_fwd(x, t, 1.0, *outs[0][:3])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    graphs = []
+    for k in (0, 1):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=streams[k]):
+            run(outs[k + 1], ds[k + 1])
+        graphs.append(gr)
+    for _ in range(3):
+        for o in outs[1] + outs[2] + ds[1:]:
+            o.fill_(3.0)
+        torch.cuda.synchronize()
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+        run(outs[0], ds[0])
+        torch.cuda.synchronize()
+        for a, b in zip(outs[1] + [ds[1]], outs[2] + [ds[2]]):
+            assert torch.equal(a, b)
+        check_fwd(x, t, 1.0, *outs[1][:3])
+        for k in (0, 3):
+            close(outs[1][k], outs[0][k].double(), 2 * sum_tol(V) + 1e-6 * outs[0][k].abs(), "logp")
+        close(ds[1], ds[0].double(), ds[0].double().abs() * 2.0 ** -6 + 1e-9, "dlogits")

@@ -34,7 +34,7 @@ INF, NAN = float("inf"), float("nan")
 CASES = [
     ("ta_token_logp_fwd", FWD, [
         (dict(N=-1), "bad shape"), (dict(V=0), "bad shape"), (dict(ld=99), "bad shape"),
-        (dict(inv_temp=F(0)), "inv_temp"), (dict(inv_temp=F(INF)), "inv_temp"),
+        (dict(V=2 ** 30 + 1, ld=2 ** 31), "bad shape"), (dict(inv_temp=F(0)), "inv_temp"), (dict(inv_temp=F(INF)), "inv_temp"),
         (dict(inv_temp=F(NAN)), "inv_temp"), (dict(logits=None), "null"),
         (dict(targets=None), "null"), (dict(logp=None), "null"), (dict(lse=None), "null"),
         (dict(logits=ODD), "misaligned")]),
@@ -47,7 +47,8 @@ CASES = [
         (dict(H=0), "bad shape"), (dict(ldh=63), "bad shape"), (dict(ldw=63), "bad shape"),
         (dict(V=0), "bad shape"), (dict(inv_temp=F(0)), "inv_temp"),
         (dict(round_logits=2), "round_logits"), (dict(h=None), "null"), (dict(h=ODD), "misaligned"),
-        (dict(ws=ctypes.c_void_p(0x1008)), "misaligned"), (dict(N=2 ** 31 - 1), "more tiles")]),
+        (dict(ws=ctypes.c_void_p(0x1008)), "misaligned"), (dict(N=2 ** 31 - 1), "more tiles"),
+        (dict(V=2 ** 30 + 1), "more tiles"), (dict(N=2 ** 25 + 1, V=1), "more tiles")]),
     ("ta_preference_loss", PREF, [
         (dict(P=-1), "bad shape"), (dict(N=-1), "bad shape"), (dict(kind=3), "kind"),
         (dict(average=2), "average"), (dict(beta=F(0)), "beta"), (dict(beta=F(NAN)), "beta"),

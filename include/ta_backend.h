@@ -135,14 +135,15 @@ int ta_token_logp_bwd_f32(const float* logits, int64_t ld, const int32_t* target
  * h [N, H] (row stride ldh) and W [V, H] (row stride ldw) BF16.  round_logits
  * 1 rounds each logit to BF16 first, as ta_gemm_bf16 writes it, so the result
  * is that of ta_token_logp_fwd on those logits up to the order of sums; 0
- * keeps them in F32.  ws: ta_lm_head_logp_ws(N, V) bytes of the caller's for
- * this call alone (16-byte aligned), or NULL: the stream's scratch pool, not
- * in a captured call.  Rows without a token give 0 (their logits are still
- * computed).  V up to 2^30, N up to 2^25.  No reference counterpart. */
+ * keeps them in F32.  ws: ta_lm_head_logp_ws(N, V, H) bytes of the caller's
+ * for this call alone (256-byte aligned), or NULL: the stream's scratch pool,
+ * not in a captured call.  Rows without a token give 0; more than 256 rows are
+ * gathered first, so those without one are not computed.  V up to 2^30, N up
+ * to 2^25.  No reference counterpart. */
 int ta_lm_head_logp(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t ldw,
                     const int32_t* targets, float inv_temp, int round_logits, float* logp,
                     float* lse, float* entropy, int N, int V, int H, void* ws, void* stream);
-int64_t ta_lm_head_logp_ws(int N, int V);
+int64_t ta_lm_head_logp_ws(int N, int V, int H);
 
 /* ── preference loss ──────────────────────────────────────────────────
  * No reference counterpart.  P pairs of packed sequences: sequence 2p is the

@@ -1119,10 +1119,9 @@ static int engine_logp(Engine* e, bool use_adapter, float* logp, float* entropy)
     int rc = forward_body(e);
     e->lora_off = false;
     CK(rc);
-    // (the logits' buffer is the workspace: it has 2 V bytes a row, the
-    // partial statistics take 3 floats per 128 columns and one more)
-    static_assert(sizeof(bf16) == 2, "");
-    void* ws = ta_lm_head_logp_ws(e->BT, e->V) <= (int64_t)e->BT * e->V * 2 ? e->logits : nullptr;
+    // (the logits' buffer, 2 V bytes a row, is the workspace where it holds it)
+    const int64_t need = ta_lm_head_logp_ws(e->BT, e->V, e->H);
+    void* ws = need <= (int64_t)e->BT * e->V * 2 ? e->logits : nullptr;
     TIMED(TA_CAT_LMHEAD, gflops(e->BT, e->V, e->H), gbytes(e->BT, e->V, e->H, 2, 0, false),
           ta_lm_head_logp(e->xfn, e->H, e->lm, e->H, e->tgt_dev, 1.f, 1, p.logp, p.lse, p.entropy,
                           e->BT, e->V, e->H, ws, e->s));

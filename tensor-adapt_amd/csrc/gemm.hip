@@ -194,18 +194,45 @@ struct TileLoader {
     }
 };
 
+// What a row-statistics launch computes: the rows with a token (lm_head_logp
+// gathers them when there is more than one tile of rows).  Their number lies
+// in device memory (ce_lse2; NULL: all M rows of X), the gathered rows, K
+// apart, at lora_u[0].  The number is taken to a scalar register, as what
+// follows from it: the stage loads take their bases from there.  (Values of
+// their own: arguments changed in place would move to memory and make the
+// product a third slower.)
+struct LseRows {
+    int M, N, K, tiles_m, tiles_n;
+    const bf16* X;
+    int64_t ldx;
+};
+__device__ __forceinline__ LseRows lse_rows(const GemmArgs& a, int BM) {
+    LseRows r = {a.M, a.N, a.K, a.tiles_m, a.tiles_n, a.X, a.ldx};
+    if (a.ce_lse2) {
+        const int live = __builtin_amdgcn_readfirstlane(*(const int32_t*)a.ce_lse2);
+        if (live < a.M) {
+            r.X = a.lora_u[0];
+            r.ldx = a.K;
+        }
+        r.M = live;
+        r.tiles_m = (live + BM - 1) / BM;
+    }
+    return r;
+}
+
 // Softmax statistics of one tile (ta_lm_head_logp): the logits are the
 // accumulators, transposed (Y rows as the MFMA's A operand): lane l of
 // acc[i][j] has row 32i + l%32 and columns 32j + 8(r/4) + 4(l/32) + r%4.  Each
 // row's (m, s, u) over the tile's columns goes to part [tiles_n][3][M], the
 // logit of the row's token, where this tile has it, to C [M].  Arguments in
 // the fields this form has free: ce_tgt the tokens, ce_inv_n = inv_temp
-// log2(e), lora_r bit 0: logits rounded to BF16 first, bit 1: u too.
+// log2(e), lora_r bit 0: logits rounded to BF16 first, bit 1: u too, ce_lse2 and
+// lora_u[0] see lse_rows.
 // A lane holds a row's 16 TN columns of its wave, the lane 32 on the others;
 // the WNW waves of a row meet in red (LDS, [WNW][BM]).
 template <int TM, int TN, int BM, int WNW, int NT>
-__device__ __forceinline__ void lse_tile(floatx16 (&acc)[TM][TN], const GemmArgs& a, int m0,
-                                         int n0, int wrow, int wn, int tn_i, int lane,
+__device__ __forceinline__ void lse_tile(floatx16 (&acc)[TM][TN], const GemmArgs& a, int M,
+                                         int m0, int n0, int wrow, int wn, int tn_i, int lane,
                                          Soft* red) {
     const int c0 = n0 + wn * TN * 32, c4 = 4 * (lane >> 5);
     const float c2 = a.ce_inv_n;
@@ -220,7 +247,7 @@ __device__ __forceinline__ void lse_tile(floatx16 (&acc)[TM][TN], const GemmArgs
 #pragma unroll
                 for (int r = 0; r < 16; r++) acc[i][j][r] = bf2f(f2bf(acc[i][j][r]));
         }
-        const int t = row < a.M ? a.ce_tgt[row] : -1;
+        const int t = row < M ? a.ce_tgt[row] : -1;
         if (t >= c0 && t < min(c0 + TN * 32, a.N)) {
             float ft = 0.f;
             bool mine = false;
@@ -259,14 +286,14 @@ __device__ __forceinline__ void lse_tile(floatx16 (&acc)[TM][TN], const GemmArgs
     }
     __syncthreads();
     for (int q = threadIdx.x; q < BM; q += NT) {
-        if (m0 + q >= a.M) break;
+        if (m0 + q >= M) break;
         Soft st = red[q];
 #pragma unroll
         for (int k = 1; k < WNW; k++) st = soft_merge(st, red[k * BM + q], c2);
-        float* P = a.part + (int64_t)tn_i * 3 * a.M + m0 + q;
+        float* P = a.part + (int64_t)tn_i * 3 * M + m0 + q;
         P[0] = st.m;
-        P[a.M] = st.s;
-        P[2 * (int64_t)a.M] = st.u;
+        P[M] = st.s;
+        P[2 * (int64_t)M] = st.u;
     }
 }
 
@@ -281,8 +308,19 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a, bool vecx, bool vecy) 
 
     // XCD-aware block order: hardware dispatches consecutive block ids
     // round-robin over 8 XCDs; give each XCD a contiguous band of tiles.
-    const int bid = xcd_band();
-    const int nt = a.tiles_m * a.tiles_n, zs = bid / nt, tile = bid - zs * nt;
+    int M = a.M, bid;
+    const bf16* X = a.X;
+    int64_t ldx = a.ldx;
+    if constexpr (EPI == EPI_LSE) {
+        const LseRows lr = lse_rows(a, BM);
+        if ((int)blockIdx.x >= lr.tiles_m * lr.tiles_n) return;
+        bid = xcd_band_of(lr.tiles_m * lr.tiles_n, blockIdx.x);
+        M = lr.M, X = lr.X, ldx = lr.ldx;
+    } else {
+        bid = xcd_band();
+    }
+    const int nt = a.tiles_m * a.tiles_n;
+    const int zs = EPI == EPI_LSE ? 0 : bid / nt, tile = bid - zs * nt;
     int tm_i = tile / a.tiles_n, tn_i = tile % a.tiles_n;
     int m0 = tm_i * BM, n0 = tn_i * BN;
     int kbeg = zs * a.k_per_split;
@@ -303,7 +341,7 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a, bool vecx, bool vecy) 
     TileLoader<BN, YK> ly;
     int nk = (kend - kbeg + BK - 1) / BK;
     if (nk > 0) {
-        lx.load(a.X, a.ldx, m0, kbeg, a.M, kend, vecx);
+        lx.load(X, ldx, m0, kbeg, M, kend, vecx);
         ly.load(a.Y, a.ldy, n0, kbeg, a.N, kend, vecy);
         lx.store(sX[0]);
         ly.store(sY[0]);
@@ -314,7 +352,7 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a, bool vecx, bool vecy) 
         bool more = kt + 1 < nk;
         if (more) {
             int k0 = kbeg + (kt + 1) * BK;
-            lx.load(a.X, a.ldx, m0, k0, a.M, kend, vecx);
+            lx.load(X, ldx, m0, k0, M, kend, vecx);
             ly.load(a.Y, a.ldy, n0, k0, a.N, kend, vecy);
         }
         const bf16* SX = sX[cur] + (wm * WTM + (lane & 31)) * LDS_STRIDE + (lane >> 5) * 8;
@@ -349,7 +387,7 @@ __global__ __launch_bounds__(256) void k_gemm(GemmArgs a, bool vecx, bool vecy) 
     if constexpr (EPI == EPI_LSE) {
         static_assert(BM * WN * sizeof(Soft) <= sizeof(sX), "row statistics fit the stages");
         // (the last k-tile's barrier is behind every read of the stages)
-        lse_tile<TM, TN, BM, WN, 256>(acc, a, m0, n0, wm * WTM, wn, tn_i, lane, (Soft*)sX);
+        lse_tile<TM, TN, BM, WN, 256>(acc, a, M, m0, n0, wm * WTM, wn, tn_i, lane, (Soft*)sX);
         return;
     }
     // epilogue: lane holds column n = lane%32 of each 32x32 tile and rows
@@ -409,8 +447,8 @@ constexpr bool tile_launch_order(int64_t M, int64_t N, int64_t K, int tiles) {
 // 1% faster than 16.  BN: the tile width of grids that tile_launch_order may
 // put in launch order (0: always ranges).
 constexpr int TILE_GM = 8;
-template <bool SPLIT, int BN>
-__device__ __forceinline__ void big_tile(const GemmArgs& a, int& tm, int& tn, int& zs) {
+template <bool SPLIT, int BN, typename Args>
+__device__ __forceinline__ void big_tile(const Args& a, int& tm, int& tn, int& zs) {
     const int nt = a.tiles_m * a.tiles_n;
     int bid;
     zs = 0;
@@ -1327,9 +1365,21 @@ __device__ __attribute__((always_inline)) inline void gemm_pipe_body(const GemmA
 
     int tm_i, tn_i;
     int zs;  // split (PART)
-    big_tile<PART, SWIGLU ? 0 : BN>(a0, tm_i, tn_i, zs);
+    LseRows lr;
+    if constexpr (LSE) {
+        lr = lse_rows(a0, BM);
+        if ((int)blockIdx.x >= lr.tiles_m * lr.tiles_n) return;
+        big_tile<false, BN>(lr, tm_i, tn_i, zs);
+    } else {
+        big_tile<PART, SWIGLU ? 0 : BN>(a0, tm_i, tn_i, zs);
+    }
     // N-concatenated groups: this tile's group supplies Y, C, N, bias, LoRA
     GemmArgs a = a0;
+    if constexpr (LSE) {
+        a.M = lr.M;
+        a.X = lr.X;
+        a.ldx = lr.ldx;
+    }
     if (a0.ngroups > 1) {
         const int g = (a0.ngroups > 2 && tn_i >= a0.tn0[2]) ? 2 : tn_i >= a0.tn0[1] ? 1 : 0;
         tn_i -= g == 2 ? a0.tn0[2] : g == 1 ? a0.tn0[1] : 0;
@@ -1697,7 +1747,7 @@ __device__ __attribute__((always_inline)) inline void gemm_pipe_body(const GemmA
     if constexpr (LSE) {
         static_assert(BM * WNW * sizeof(Soft) <= sizeof(sXs), "row statistics fit the stages");
         __syncthreads();  // every wave is done with the stage buffers
-        lse_tile<TM, TN, BM, WNW, NW * 64>(acc, a, m0, n0, wm * WTM, wn, tn_i, lane, (Soft*)sXs);
+        lse_tile<TM, TN, BM, WNW, NW * 64>(acc, a, lr.M, m0, n0, wm * WTM, wn, tn_i, lane, (Soft*)sXs);
         return;
     }
 #undef PIPE_CE
@@ -3074,7 +3124,11 @@ __global__ __launch_bounds__(1024) void k_lse_merge(const float* __restrict__ pa
                                                     const int32_t* __restrict__ targets, float c,
                                                     float* __restrict__ logp,
                                                     float* __restrict__ lse,
-                                                    float* __restrict__ entropy, int N, int V) {
+                                                    float* __restrict__ entropy, int N, int V,
+                                                    const int32_t* __restrict__ live,
+                                                    const int32_t* __restrict__ rows) {
+    if (live) N = *live;
+    if (blockIdx.x * (int64_t)R >= N) return;
     constexpr int LPR = 1024 / R, U = 8;
     __shared__ float redm[16][R];
     __shared__ double red[16][R][2];
@@ -3129,20 +3183,116 @@ __global__ __launch_bounds__(1024) void k_lse_merge(const float* __restrict__ pa
     const int t = targets[row];
     RowOut o = {0.0, 0.f, 0.f};
     if (t >= 0) o = row_out(st, t < V ? tlogit[row] : 0.f, t < V, c);
-    logp[row] = (float)o.logp;
-    lse[row] = o.lse;
-    if (entropy) entropy[row] = o.ent;
+    const int64_t to = rows ? (int64_t)rows[row] : row;
+    logp[to] = (float)o.logp;
+    lse[to] = o.lse;
+    if (entropy) entropy[to] = o.ent;
 }
 
-// bytes of partial statistics and token logits: no form has tiles narrower
-// than 128 columns
-int64_t lm_head_logp_ws(int N, int V) {
-    return ((int64_t)((V + 127) / 128) * 3 + 1) * N * (int64_t)sizeof(float);
+// The rows with a token, in order: rows and their tokens, *live their number.
+// Rows without one get their zeros here.  One block, 8192 rows a sweep (5 us):
+// a wave takes 512 in a row, 64 at a time, whose ballots say where they go.
+__global__ __launch_bounds__(1024) void k_live_rows(const int32_t* __restrict__ targets, int N,
+                                                    int32_t* __restrict__ rows,
+                                                    int32_t* __restrict__ tokens,
+                                                    int32_t* __restrict__ live,
+                                                    float* __restrict__ logp,
+                                                    float* __restrict__ lse,
+                                                    float* __restrict__ entropy) {
+    __shared__ int sums[16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    int base = 0;
+    for (int r0 = 0; r0 < N; r0 += 8192) {
+        const int r = r0 + 512 * w + lane;
+        int t[8], c = 0;
+        uint64_t on[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) t[i] = r + 64 * i < N ? targets[r + 64 * i] : -1;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            on[i] = __ballot(t[i] >= 0);
+            c += __popcll(on[i]);
+        }
+        __syncthreads();  // sums is read
+        if (lane == 0) sums[w] = c;
+        __syncthreads();
+        // the waves before this one, and all
+        int all = lane < 16 ? sums[lane] : 0, at = lane < w ? all : 0;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+            at += __shfl_xor(at, o, 64), all += __shfl_xor(all, o, 64);
+        at = base + __shfl(at, 0, 64);
+        base += __shfl(all, 0, 64);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int q = r + 64 * i;
+            if (t[i] >= 0) {
+                const int to = at + __popcll(on[i] & below);
+                rows[to] = q;
+                tokens[to] = t[i];
+            } else if (q < N) {
+                logp[q] = 0.f;
+                lse[q] = 0.f;
+                if (entropy) entropy[q] = 0.f;
+            }
+            at += __popcll(on[i]);
+        }
+    }
+    if (threadIdx.x == 0) *live = base;
+}
+// X [*live, H] = the rows of h that have a token; nothing if all have.  A wave
+// per row.
+__global__ __launch_bounds__(256) void k_gather_rows(const bf16* __restrict__ h, int64_t ldh,
+                                                     const int32_t* __restrict__ rows,
+                                                     const int32_t* __restrict__ live, int N,
+                                                     int H, bool vec, bf16* __restrict__ X) {
+    const int64_t r = blockIdx.x * 4ll + (threadIdx.x >> 6);
+    const int n = *live, lane = threadIdx.x & 63;
+    if (r >= n || n == N) return;
+    const bf16* src = h + (int64_t)rows[r] * ldh;
+    bf16* dst = X + r * H;
+    if (vec)
+        for (int k = lane; k < H / 8; k += 64) ((bf16x8v*)dst)[k] = ((const bf16x8v*)src)[k];
+    else
+        for (int k = lane; k < H; k += 64) dst[k] = src[k];
+}
+
+// Whether the rows with a token are gathered: with one tile of rows they
+// would not be fewer.  A prompt's rows are then not computed (4096 x 151,936 x
+// 1536 with 40% of the rows masked 1672 -> 1068 us, 2048 rows 840 -> 500); where
+// all have a token nothing is copied and the two launches and the number's
+// load in each tile cost 1% (8192 rows 3238 -> 3270 us) to 3% (512 rows 240 ->
+// 247).
+static bool lse_gathers(int N) { return N > 256; }
+// The workspace: token logits [N], partial statistics (no form has tiles
+// narrower than 128 columns), then the live rows' number, indices and tokens
+// and the gathered rows.
+struct LseWs {
+    int64_t part, live, x, bytes;
+};
+static LseWs lse_ws(int N, int V, int H) {
+    LseWs w{};
+    auto up = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
+    w.part = up((int64_t)N * 4);
+    w.live = w.part + up((int64_t)((V + 127) / 128) * 3 * N * 4);
+    w.x = w.bytes = w.live;
+    if (lse_gathers(N)) {
+        w.x = w.live + up((2 * (int64_t)N + 64) * 4);
+        w.bytes = w.x + up((int64_t)N * H * 2);
+    }
+    return w;
 }
 
 int lm_head_logp(const bf16* h, int64_t ldh, const bf16* W, int64_t ldw, const int32_t* targets,
                  float c, bool round, float* logp, float* lse, float* entropy, int N, int V, int H,
                  void* ws, hipStream_t s) {
+    const LseWs lay = lse_ws(N, V, H);
+    if (!ws) {
+        // (two graphs of one stream would share the pool's buffer)
+        TA_REQUIRE(!is_capturing(s), "lm_head_logp: a captured call needs a workspace of its own");
+        if (int rc = scratch_here("lm_head_logp", (size_t)lay.bytes, s, &ws)) return rc;
+    }
     GemmArgs a{};
     a.M = N;
     a.N = V;
@@ -3156,14 +3306,22 @@ int lm_head_logp(const bf16* h, int64_t ldh, const bf16* W, int64_t ldw, const i
     a.ce_tgt = targets;
     a.ce_inv_n = c * kLog2e;
     a.lora_r = (round ? 1 : 0) | (entropy ? 2 : 0);
-    if (!ws) {
-        // (two graphs of one stream would share the pool's buffer)
-        TA_REQUIRE(!is_capturing(s), "lm_head_logp: a captured call needs a workspace of its own");
-        if (int rc = scratch_here("lm_head_logp", (size_t)lm_head_logp_ws(N, V), s, &ws)) return rc;
-    }
     a.C = ws;
-    a.part = (float*)ws + N;
-    const bool vx = al16(h) && ldh % 8 == 0, vw = al16(W) && ldw % 8 == 0;
+    a.part = (float*)((char*)ws + lay.part);
+    const bool vx = al16(h) && ldh % 8 == 0 && H % 8 == 0, vw = al16(W) && ldw % 8 == 0;
+    int32_t *live = nullptr, *rows = nullptr;
+    if (lse_gathers(N)) {
+        live = (int32_t*)((char*)ws + lay.live);
+        rows = live + 64;
+        int32_t* tokens = rows + N;
+        bf16* X = (bf16*)((char*)ws + lay.x);
+        tlaunch(k_live_rows, dim3(1), dim3(1024), s, targets, N, rows, tokens, live, logp, lse,
+                entropy);
+        tlaunch(k_gather_rows, dim3((N + 3) / 4), dim3(256), s, h, ldh, rows, live, N, H, vx, X);
+        a.ce_lse2 = (const float*)live;
+        a.lora_u[0] = X;
+        a.ce_tgt = tokens;
+    }
     const bool pipe = H % BK == 0 && vx && vw && ldh < kMaxStageLd && ldw < kMaxStageLd;
     // 256-row tiles where 128-row ones would read W twice (151,936 x 1536, us:
     // 128 rows 133 against 150, 129 rows 159 against 151, 256 rows 184 against
@@ -3180,10 +3338,10 @@ int lm_head_logp(const bf16* h, int64_t ldh, const bf16* W, int64_t ldw, const i
         tlaunch(k_gemm<128, 128, 2, 2, true, true, EPI_LSE>, grid, dim3(256), s, a, vx, vw);
     if (N <= 1024)
         tlaunch(k_lse_merge<4>, dim3((N + 3) / 4), dim3(1024), s, a.part, a.tiles_n,
-                (const float*)a.C, targets, c, logp, lse, entropy, N, V);
+                (const float*)a.C, a.ce_tgt, c, logp, lse, entropy, N, V, live, rows);
     else
         tlaunch(k_lse_merge<16>, dim3((unsigned)(((int64_t)N + 15) / 16)), dim3(1024), s, a.part,
-                a.tiles_n, (const float*)a.C, targets, c, logp, lse, entropy, N, V);
+                a.tiles_n, (const float*)a.C, a.ce_tgt, c, logp, lse, entropy, N, V, live, rows);
     return check_launch("lm_head_logp");
 }
 
@@ -3237,8 +3395,8 @@ int ta_gemm_rm(int x_kmajor, int y_kmajor, int M, int N, int K, float alpha, con
                          ldc, bias, (hipStream_t)stream, 0, nullptr);
 }
 
-int64_t ta_lm_head_logp_ws(int N, int V) {
-    return N > 0 && V > 0 ? lm_head_logp_ws(N, V) : 0;
+int64_t ta_lm_head_logp_ws(int N, int V, int H) {
+    return N > 0 && V > 0 && H > 0 ? lse_ws(N, V, H).bytes : 0;
 }
 
 int ta_lm_head_logp(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t ldw,
@@ -3254,7 +3412,7 @@ int ta_lm_head_logp(const uint16_t* h, int64_t ldh, const uint16_t* W, int64_t l
                "lm_head_logp: N=%d x V=%d takes more tiles than a launch", N, V);
     if (N == 0) return 0;
     TA_REQUIRE(h && W && targets && logp && lse, "lm_head_logp: null argument");
-    TA_REQUIRE((((uintptr_t)h | (uintptr_t)W) & 1) == 0 && ((uintptr_t)ws & 15) == 0,
+    TA_REQUIRE((((uintptr_t)h | (uintptr_t)W) & 1) == 0 && ((uintptr_t)ws & 255) == 0,
                "lm_head_logp: misaligned operand");
     return lm_head_logp(h, ldh, W, ldw, targets, inv_temp, round_logits != 0, logp, lse, entropy, N,
                         V, H, ws, (hipStream_t)stream);

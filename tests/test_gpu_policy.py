@@ -261,7 +261,7 @@ def test_lm_head_logp(N, V, H):
         # dH = -sum p (log p + H) dx: at most 2 (log V + 1) max|dx|
         close(o[2], we, 4 * (math.log(V) + 2) * tol, "entropy")
         # the caller's workspace, without the entropy: the same bits
-        ws_ = torch.empty(tadapt.lib().ta_lm_head_logp_ws(N, V), device=DEV, dtype=torch.uint8)
+        ws_ = torch.empty(tadapt.lib().ta_lm_head_logp_ws(N, V, H), device=DEV, dtype=torch.uint8)
         o2 = [full(N) for _ in range(2)]
         call("ta_lm_head_logp", P(h), H + pad, P(W), H + pad, P(t), F(c), 0, *map(P, o2), None, N,
              V, H, P(ws_), S())
@@ -280,6 +280,32 @@ def test_lm_head_logp(N, V, H):
         close(o[0], p2[0], step + 2 * tol, "logp, rounded")
         frac = ((o[0] - p2[0]).abs() > 0.1 * step + 2 * tol).double().mean()
         assert N < 64 or frac < 0.05, frac
+
+
+@pytest.mark.parametrize("N,H,pad", [(257, 64, 0), (700, 192, 8), (1300, 100, 3), (5000, 64, 0)])
+@pytest.mark.parametrize("masked", [0.0, 0.4, 0.97, 1.0])
+def test_lm_head_logp_masked_rows(N, H, pad, masked):
+    """Rows without a token are left out of the product, wherever they lie;
+    what the others give does not depend on them."""
+    V = 1501
+    g = gen(N + H)
+    h = randn(g, N, H + pad, dtype=BF16)[:, :H]
+    W = randn(g, V, H, std=2.0 / math.sqrt(H), dtype=BF16)
+    every = tokens(g, N, V, 0.0)
+    t = torch.where(torch.rand(N, generator=g, device=DEV) < masked, torch.full_like(every, -5), every)
+    if masked == 0.4:  # a prompt at the start, padding at the end, the last row alone
+        t[:200] = -1
+        t[N - 90:N - 1] = -1
+        t[N - 1] = 7
+        every[N - 1] = 7
+    h.masked_fill_((t < 0)[:, None], NAN)
+    want, o = [full(N) for _ in range(3)], [full(N) for _ in range(3)]
+    call("ta_lm_head_logp", P(h), H + pad, P(W), H, P(every), F(1), 0, *map(P, want), N, V, H, None,
+         S())
+    call("ta_lm_head_logp", P(h), H + pad, P(W), H, P(t), F(1), 0, *map(P, o), N, V, H, None, S())
+    on = t >= 0
+    for a, b in zip(o, want):
+        assert (a[~on] == 0).all() and torch.equal(a[on], b[on])
 
 
 def test_lm_head_logp_infinite_inputs():
@@ -675,7 +701,7 @@ def test_lm_head_logp_captured_twice():
     W = randn(g, V, H, std=2 / math.sqrt(H), dtype=BF16)
     hs = [randn(g, N, H, dtype=BF16) for _ in range(2)]
     t = tokens(g, N, V, 0.0)
-    need = tadapt.lib().ta_lm_head_logp_ws(N, V)
+    need = tadapt.lib().ta_lm_head_logp_ws(N, V, H)
     ws = [torch.empty(need, device=DEV, dtype=torch.uint8) for _ in range(2)]
     outs = [[full(N) for _ in range(3)] for _ in range(2)]
     graphs = []

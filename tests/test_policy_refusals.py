@@ -89,5 +89,7 @@ def test_nothing_to_do(name, good, empty):
 
 def test_workspace_size():
     L = tadapt.lib()
-    assert L.ta_lm_head_logp_ws(0, 100) == 0
-    assert L.ta_lm_head_logp_ws(5, 129) == (2 * 3 + 1) * 5 * 4
+    assert L.ta_lm_head_logp_ws(0, 100, 64) == 0
+    small, large = L.ta_lm_head_logp_ws(5, 129, 64), L.ta_lm_head_logp_ws(300, 129, 64)
+    assert small >= (2 * 3 + 1) * 5 * 4 and small % 256 == 0
+    assert large >= (2 * 3 + 1) * 300 * 4 + 300 * 64 * 2 + 2 * 300 * 4

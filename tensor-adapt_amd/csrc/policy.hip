@@ -147,6 +147,14 @@ struct GradRow {
     int t;
     float c, lse, H, g, e;
 };
+// the same for every lane: taken to scalar registers
+__device__ __forceinline__ float uniform_f(float f) {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(f)));
+}
+__device__ __forceinline__ GradRow uniform_row(const GradRow& r) {
+    return {__builtin_amdgcn_readfirstlane(r.t), uniform_f(r.c), uniform_f(r.lse),
+            uniform_f(r.H),                      uniform_f(r.g), uniform_f(r.e)};
+}
 template <typename T, bool NT>
 __device__ __forceinline__ void span_grad_ld(const T* L, T* D, const Span& sp, const GradRow& r,
                                              int tid, int nt) {
@@ -313,13 +321,13 @@ __device__ __forceinline__ void policy_no_row(const PolicyRows& r, int64_t n) {
     if (r.kl) r.kl[n] = 0.f;
 }
 
-// Two passes over the row, the second out of the caches: short rows, for
-// which a 1024-thread block is too wide, and those too long for its registers
-// (2048 x 151,936, a quarter without a token: 280 us, 233 in registers).
-template <int NW, bool ENT>
-__global__ __launch_bounds__(64 * NW) void k_policy_logits(PolicyRows r, PolicyArgs a) {
-    __shared__ float redm[NW];
-    __shared__ double red[NW][2];
+// Two passes over the row, the second out of the caches: for rows too long for
+// a block's registers (2048 x 151,936, a quarter without a token: 280 us, 233
+// in registers).
+template <bool ENT>
+__global__ __launch_bounds__(512) void k_policy_logits(PolicyRows r, PolicyArgs a) {
+    __shared__ float redm[8];
+    __shared__ double red[8][2];
     __shared__ GradRow sg;
     const Span sp = span_of<bf16>(r.V, 0, 1);
     for (int64_t n = blockIdx.x; n < r.N; n += gridDim.x) {
@@ -329,24 +337,24 @@ __global__ __launch_bounds__(64 * NW) void k_policy_logits(PolicyRows r, PolicyA
         if (w != 0.f) {
             const int t = r.targets[n];
             const float ft = t < r.V ? bf2f(L[t]) : 0.f;
-            const SoftRow st = span_soft<bf16, NW, ENT>(r.nt, L, sp, r.c * kLog2e, redm, red);
+            const SoftRow st = span_soft<bf16, 8, ENT>(r.nt, L, sp, r.c * kLog2e, redm, red);
             if (threadIdx.x == 0) sg = policy_row(r, a, n, st, ft, w);
             __syncthreads();
-            span_grad(r.nt, L, D, sp, sg, threadIdx.x, 64 * NW);
+            span_grad(r.nt, L, D, sp, sg, threadIdx.x, 512);
         } else {
-            span_zero(D, sp, threadIdx.x, 64 * NW);
+            span_zero(D, sp, threadIdx.x, 512);
             if (threadIdx.x == 0) policy_no_row(r, n);
         }
         __syncthreads();  // sg is read before the next row writes it
     }
 }
 
-// A row held in the registers of its 1024-thread block, so that it is read
-// once: up to CPT whole sweeps of 1024 vectors, the part sweep after them and
-// the V % E values past the vectors (CPT <= 19 of BF16: 80 of a lane's 128
-// registers).  Whether a sweep is whole is the same for every lane, so it
-// costs no lane mask and one address register for all of them.
-template <typename T, int CPT>
+// A row held in the registers of its block of NT threads, so that it is read
+// once: up to CPT whole sweeps of NT vectors, the part sweep after them and the
+// V % E values past the vectors (CPT <= 19 of BF16: 80 registers of a lane,
+// where a 1024-thread block has 128).  Whether a sweep is whole is the same for
+// every lane, so it costs no lane mask and one address register for all.
+template <typename T, int CPT, int NT>
 struct RegRow {
     typedef typename Row<T>::V4 V4;
     static constexpr int E = Row<T>::E;
@@ -356,21 +364,22 @@ struct RegRow {
     int tail;         // index of this lane's value past the vectors, or -1
     __device__ __forceinline__ void load(const T* L, int V, bool nt) {
         const int nv = V / E, it = nv * E + (int)threadIdx.x;
-        whole = nv >> 10;
-        part = nv & 1023;
+        whole = nv / NT;
+        part = nv % NT;
         tail = it < V ? it : -1;
         if (nt) {
 #pragma unroll
             for (int k = 0; k < CPT; k++)
-                    if (k < whole) v[k] = Row<T>::template ld<true>(L + ((int64_t)k * 1024 + threadIdx.x) * E);
+                    if (k < whole)
+                    v[k] = Row<T>::template ld<true>(L + (int64_t)k * NT * E + threadIdx.x * E);
         } else {
 #pragma unroll
             for (int k = 0; k < CPT; k++)
                 if (k < whole)
-                    v[k] = Row<T>::template ld<false>(L + (int64_t)k * 1024 * E + threadIdx.x * E);
+                    v[k] = Row<T>::template ld<false>(L + (int64_t)k * NT * E + threadIdx.x * E);
         }
         if ((int)threadIdx.x < part)
-            vp = Row<T>::template ld<false>(L + (int64_t)whole * 1024 * E + threadIdx.x * E);
+            vp = Row<T>::template ld<false>(L + (int64_t)whole * NT * E + threadIdx.x * E);
         ft = tail >= 0 ? Row<T>::one(L + tail) : 0.f;
     }
     // f(values, first index) for every vector of the lane.  The empty asm
@@ -384,24 +393,24 @@ struct RegRow {
                 asm volatile("" : "+v"(v[k]));
                 float x[E];
                 Row<T>::unpack(v[k], x);
-                f(x, k * 1024 + (int)threadIdx.x);
+                f(x, k * NT + (int)threadIdx.x, k);
                 __builtin_amdgcn_sched_barrier(0);  // one vector's temporaries at a time
             }
         if ((int)threadIdx.x < part) {
             asm volatile("" : "+v"(vp));
             float x[E];
             Row<T>::unpack(vp, x);
-            f(x, whole * 1024 + (int)threadIdx.x);
+            f(x, whole * NT + (int)threadIdx.x, whole);
         }
     }
     template <bool ENT>
     __device__ __forceinline__ SoftRow soft(float c2, float* redm, double (*red)[2]) {
         float m = tail >= 0 ? ft : -INFINITY;
-        each([&](const float* x, int) {
+        each([&](const float* x, int, int) {
 #pragma unroll
             for (int e = 0; e < E; e++) m = fmaxf(m, x[e]);
         });
-        m = block_maxf<16>(m, redm);
+        m = block_maxf<NT / 64>(m, redm);
         const float R = soft_ref(m);
         float s = 0.f, u = 0.f;
         auto add = [&](float x) {
@@ -410,40 +419,40 @@ struct RegRow {
             if (ENT) u = fmaf(p, fmaxf(d, kFar), u);
         };
         if (tail >= 0) add(ft);
-        each([&](const float* x, int) {
+        each([&](const float* x, int, int) {
 #pragma unroll
             for (int e = 0; e < E; e++) add(x[e]);
         });
-        return block_sums<16, ENT>(m, s, u, red);
+        return block_sums<NT / 64, ENT>(m, s, u, red);
     }
 };
 
-template <int CPT, bool ENT>
-__global__ __launch_bounds__(1024) void k_policy_reg(PolicyRows r, PolicyArgs a) {
-    __shared__ float redm[16];
-    __shared__ double red[16][2];
+template <int CPT, int NT, bool ENT>
+__global__ __launch_bounds__(NT) void k_policy_reg(PolicyRows r, PolicyArgs a) {
+    __shared__ float redm[NT / 64];
+    __shared__ double red[NT / 64][2];
     __shared__ GradRow sg;
     const int64_t n = blockIdx.x;
     const float w = row_weight(r, a, n);
     const bf16* L = r.logits + n * r.ld;
     bf16* D = r.dlogits + n * r.ldd;
     if (w == 0.f) {
-        span_zero(D, span_of<bf16>(r.V, 0, 1), threadIdx.x, 1024);
+        span_zero(D, span_of<bf16>(r.V, 0, 1), threadIdx.x, NT);
         if (threadIdx.x == 0) policy_no_row(r, n);
         return;
     }
     // (every load of the row is before the block's barriers, which the stores
     // to dlogits, maybe the same row, are behind)
-    RegRow<bf16, CPT> row;
+    RegRow<bf16, CPT, NT> row;
     row.load(L, r.V, r.nt);
     const int t = r.targets[n];
     const float ft = t < r.V ? bf2f(L[t]) : 0.f;
     const SoftRow st = row.template soft<ENT>(r.c * kLog2e, redm, red);
     if (threadIdx.x == 0) sg = policy_row(r, a, n, st, ft, w);
     __syncthreads();
-    const GradRow g = sg;
+    const GradRow g = uniform_row(sg);
     const int tc = g.t >> 3;
-    row.each([&](const float* x, int q) {
+    row.each([&](const float* x, int q, int k) {
         float f[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) f[i] = logit_grad<ENT>(x[i], g.c, g.lse, g.H, g.g, g.e);
@@ -451,8 +460,7 @@ __global__ __launch_bounds__(1024) void k_policy_reg(PolicyRows r, PolicyArgs a)
 #pragma unroll
             for (int i = 0; i < 8; i++) f[i] += i == (g.t & 7) ? g.c * g.g : 0.f;
         }
-        const int k = q >> 10;  // (a constant or the same for every lane)
-        Row<bf16>::store(D + (int64_t)k * 8192 + 8 * threadIdx.x, f);
+        Row<bf16>::store(D + (int64_t)k * NT * 8 + 8 * threadIdx.x, f);
     });
     if (row.tail >= 0)
         D[row.tail] = f2bf(logit_grad<ENT>(row.ft, g.c, g.lse, g.H, g.g, g.e) +
@@ -655,11 +663,16 @@ static inline dim3 row_grid(int64_t rows) { return dim3((unsigned)(rows < (1 << 
 constexpr int kMaxV = 1 << 30;  // indices into a row stay below 2^31
 static bool temp_ok(float c) { return c > 0.f && c < INFINITY; }
 
-// Whether rows take a block of two waves instead of eight: where eight have
-// hardly a vector per lane, and where many rows share a CU anyway (2048 rows
-// of 1000, forward 8.1 -> 4.2 us and gradient 6.4 -> 4.2; of 8000, forward 12.4
-// -> 10.1, policy step 31 -> 20; but one row of 8000, 3.0 -> 4.0).
-static bool narrow(int N, int V) { return V <= 2048 || (N >= 1024 && V <= 12288); }
+// Waves of a row's block in the forward: narrow ones where the row has hardly a
+// vector per lane of eight waves, and where there are many rows to share a CU
+// (us, 2 / 4 / 8 waves: 2000 rows of 1000 4.2 / 5.2 / 7.9, of 8000 11.0 / 9.8 /
+// 11.7; 100 rows of 8000 5.6 / 4.4 / 3.9).
+static int fwd_waves(int N, int V) {
+    return V <= 2048 ? 2 : V <= 4096 || (V <= 12288 && N >= 512) ? 4 : 8;
+}
+// Threads of a gradient's block (128 / 256 / 512, us: 2000 rows of 1000 4.2 /
+// 4.9 / 6.4, of 4000 9.0 / 8.4 / 8.8, of 8000 15.3 / 14.6 / 13.7).
+static int bwd_threads(int V) { return V <= 1024 ? 128 : V <= 4096 ? 256 : 512; }
 
 // Blocks that each row's statistics are split over (1: one block per row,
 // also in a capture, where graphs of one stream would share the parts).  One
@@ -712,9 +725,13 @@ static int token_logp_fwd(const T* logits, int64_t ld, const int32_t* targets, f
 #define TL(NW, ENT)                                                                             \
     tlaunch(k_token_logp<T, NW, ENT>, row_grid(N), dim3(64 * NW), s, logits, ld, targets, c,    \
             logp, lse, entropy, N, V, nt)
-    if (narrow(N, V)) {
+    const int nw = fwd_waves(N, V);
+    if (nw == 2) {
         if (entropy) TL(2, true);
         else TL(2, false);
+    } else if (nw == 4) {
+        if (entropy) TL(4, true);
+        else TL(4, false);
     } else {
         if (entropy) TL(8, true);
         else TL(8, false);
@@ -739,7 +756,7 @@ static int token_logp_bwd(const T* logits, int64_t ld, const int32_t* targets, f
                "token_logp_bwd: misaligned rows");
     TA_REQUIRE(dlogits != logits || ldd == ld, "token_logp_bwd: in place needs ldd = ld");
     const int splits = grad_splits(N, V, sizeof(T));
-    tlaunch(k_token_logp_bwd<T>, row_grid((int64_t)N * splits), dim3(V <= 2048 ? 128 : 512), s,
+    tlaunch(k_token_logp_bwd<T>, row_grid((int64_t)N * splits), dim3(bwd_threads(V)), s,
             logits, ld, targets, c, lse, entropy, dlogp, dentropy, dlogits, ldd, N, V, splits,
             (int64_t)N * V * (int64_t)sizeof(T) > kCacheBytes);
     return check_launch("token_logp_bwd");
@@ -879,30 +896,47 @@ int ta_policy_loss_logits(const uint16_t* logits, int64_t ld, const int32_t* tar
         tlaunch(k_policy_grad, grid, dim3(512), s, r, grads, splits);
         return check_launch("policy_loss_logits");
     }
-    // in registers from two whole sweeps of a 1024-thread block on (2048 rows of
-    // 16,384: 39 us, in two passes 47; of 12,000: 32 and, two waves a row, 31)
-    const int sweeps = V / 8 / 1024;
-    if (sweeps >= 2 && sweeps <= 19 && N <= (1 << 20)) {
-#define PL(C)                                                           \
-    if (entropy)                                                        \
-        tlaunch(k_policy_reg<C, true>, dim3(N), dim3(1024), s, r, a);   \
-    else                                                                \
-        tlaunch(k_policy_reg<C, false>, dim3(N), dim3(1024), s, r, a)
-        if (sweeps <= 3) { PL(3); }
-        else if (sweeps <= 7) { PL(7); }
-        else if (sweeps <= 15) { PL(15); }
-        else { PL(19); }
-#undef PL
-    } else {
-#define PL(NW, ENT) tlaunch(k_policy_logits<NW, ENT>, row_grid(N), dim3(64 * NW), s, r, a)
-        if (narrow(N, V)) {
-            if (entropy) PL(2, true);
-            else PL(2, false);
+    // Rows in registers: the narrowest block that holds the row lets the most
+    // rows share a CU, whose loads, sums and stores then overlap (2000 rows, us,
+    // blocks of 128 / 256 / 512 / 1024 threads: of 1000 logits 6.6 / 8.3 / 12.6 /
+    // 22.7, of 16,000 30 / 30 / 30 / 38, of 40,000 - / 66 / 71 / 90, of 80,000 - /
+    // - / 127 / 157); few rows are faster in wider ones (100 of 16,000 10.3 / 7.7
+    // / 7.4 / 7.6).
+    const int nt = V <= 2048                                ? 128
+                   : V <= 8192 || (V < 40960 && N >= 1000) ? 256
+                   : V < 81920                              ? 512
+                                                            : 1024;
+    const int sweeps = V / 8 / nt;
+    if (sweeps <= 19 && N <= (1 << 20)) {
+#define PL(C, NT)                                                           \
+    do {                                                                    \
+        if (entropy)                                                        \
+            tlaunch(k_policy_reg<C, NT, true>, dim3(N), dim3(NT), s, r, a); \
+        else                                                                \
+            tlaunch(k_policy_reg<C, NT, false>, dim3(N), dim3(NT), s, r, a); \
+    } while (0)
+#define PL4(NT)                    \
+    if (sweeps <= 3) PL(3, NT);    \
+    else if (sweeps <= 7) PL(7, NT); \
+    else if (sweeps <= 15) PL(15, NT); \
+    else PL(19, NT)
+        if (nt == 128) {
+            PL(3, 128);
+        } else if (nt == 256) {
+            PL4(256);
+        } else if (nt == 512) {
+            PL4(512);
+        } else if (sweeps <= 15) {
+            PL(15, 1024);
         } else {
-            if (entropy) PL(8, true);
-            else PL(8, false);
+            PL(19, 1024);
         }
+#undef PL4
 #undef PL
+    } else if (entropy) {
+        tlaunch(k_policy_logits<true>, row_grid(N), dim3(512), s, r, a);
+    } else {
+        tlaunch(k_policy_logits<false>, row_grid(N), dim3(512), s, r, a);
     }
     return check_launch("policy_loss_logits");
 }

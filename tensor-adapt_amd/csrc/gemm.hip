@@ -3284,6 +3284,18 @@ static LseWs lse_ws(int N, int V, int H) {
     return w;
 }
 
+// Whether 256 x 256 tiles, one a CU, take less time than 128 x 128 ones, two a
+// CU: a wave of 512 of these takes about 0.61 of a wave of 256 of those.
+// Measured, 128 / 256, us at H = 1536: 1024 x 8000 (1 wave each) 38 / 47, 2048 x
+// 8000 (2, 1) 64 / 58, 256 x 80,000 (3, 2) 76 / 86, 1024 x 50,257 (7, 4) 174 /
+// 176, 256 x 151,936 (5, 3) 184 / 164, 8192 x 151,936 3820 / 3170.
+static bool lse_big_tiles(int N, int V) {
+    auto waves = [&](int64_t t, int64_t slots) {
+        return (((N + t - 1) / t) * ((V + t - 1) / t) + slots - 1) / slots;
+    };
+    return 100 * waves(256, 256) <= 61 * waves(128, 512);
+}
+
 int lm_head_logp(const bf16* h, int64_t ldh, const bf16* W, int64_t ldw, const int32_t* targets,
                  float c, bool round, float* logp, float* lse, float* entropy, int N, int V, int H,
                  void* ws, hipStream_t s) {
@@ -3323,10 +3335,7 @@ int lm_head_logp(const bf16* h, int64_t ldh, const bf16* W, int64_t ldw, const i
         a.ce_tgt = tokens;
     }
     const bool pipe = H % BK == 0 && vx && vw && ldh < kMaxStageLd && ldw < kMaxStageLd;
-    // 256-row tiles where 128-row ones would read W twice (151,936 x 1536, us:
-    // 128 rows 133 against 150, 129 rows 159 against 151, 256 rows 184 against
-    // 164, 8192 rows 3820 against 3170)
-    const int bt = pipe && N > 128 ? 256 : 128;
+    const int bt = pipe && lse_big_tiles(N, V) ? 256 : 128;
     a.tiles_m = (N + bt - 1) / bt;
     a.tiles_n = (V + bt - 1) / bt;
     const dim3 grid(a.tiles_m * a.tiles_n);

@@ -370,7 +370,7 @@ struct RegRow {
         if (nt) {
 #pragma unroll
             for (int k = 0; k < CPT; k++)
-                    if (k < whole)
+                if (k < whole)
                     v[k] = Row<T>::template ld<true>(L + (int64_t)k * NT * E + threadIdx.x * E);
         } else {
 #pragma unroll

@@ -216,6 +216,25 @@ def test_special_logits(V, dtype):
     assert (d[1] == 0).all() and torch.isfinite(d[6]).all()
 
 
+def test_more_rows_than_blocks():
+    """Past 2^20 rows a block takes several."""
+    N, V = (1 << 20) + 37, 5
+    g = gen(6)
+    x, t = rows(g, N, V, BF16), tokens(g, N, V, 0.2)
+    o = [full(N) for _ in range(3)]
+    call("ta_token_logp_fwd", P(x), V, P(t), F(1), *map(P, o), N, V, S())
+    check_fwd(x, t, 1.0, *o)
+    dl, d = randn(g, N), torch.empty_like(x)
+    call("ta_token_logp_bwd", P(x), V, P(t), F(1), P(o[1]), None, P(dl), None, P(d), V, N, V, S())
+    check_bwd(x, t, 1.0, d, dl, None, V)
+    # (old_logp NULL, no KL term: dlogp = -adv * weight)
+    adv, w = randn(g, N), torch.rand(N, generator=g, device=DEV)
+    q = [full(N) for _ in range(4)]
+    call("ta_policy_loss_logits", P(x), V, P(t), F(1), None, None, P(adv), P(w), F(0.2), F(0.2),
+         F(0), F(0), F(0), *map(P, q), P(d), V, N, V, S())
+    check_bwd(x, t, 1.0, d, -adv * w, None, V)
+
+
 @pytest.mark.parametrize("sfx", ["", "_f32"])
 def test_rows_far_apart(sfx):
     """Row offsets past 2^31 elements."""
@@ -237,7 +256,8 @@ def test_rows_far_apart(sfx):
 
 # ── LM head scoring ────────────────────────────────────────────────────────
 HEADS = [(1, 1, 1), (1, 1000, 64), (3, 257, 7), (64, 128, 128), (130, 2049, 96), (65, 5000, 200),
-         (300, 3001, 256), (257, 1537, 64), (1, 151936, 896), (17, 32000, 512), (512, 20000, 1536)]
+         (300, 3001, 256), (257, 1537, 64), (1, 151936, 896), (17, 32000, 512), (512, 20000, 1536),
+         (700, 40001, 128)]
 
 
 @pytest.mark.parametrize("N,V,H", HEADS)
@@ -282,12 +302,13 @@ def test_lm_head_logp(N, V, H):
         assert N < 64 or frac < 0.05, frac
 
 
-@pytest.mark.parametrize("N,H,pad", [(257, 64, 0), (700, 192, 8), (1300, 100, 3), (5000, 64, 0)])
+@pytest.mark.parametrize("N,V,H,pad", [(257, 1501, 64, 0), (700, 1501, 192, 8),
+                                       (1300, 1501, 100, 3), (9000, 1501, 64, 0),
+                                       (1300, 30011, 64, 0)])  # the last in 256 x 256 tiles
 @pytest.mark.parametrize("masked", [0.0, 0.4, 0.97, 1.0])
-def test_lm_head_logp_masked_rows(N, H, pad, masked):
+def test_lm_head_logp_masked_rows(N, V, H, pad, masked):
     """Rows without a token are left out of the product, wherever they lie;
     what the others give does not depend on them."""
-    V = 1501
     g = gen(N + H)
     h = randn(g, N, H + pad, dtype=BF16)[:, :H]
     W = randn(g, V, H, std=2.0 / math.sqrt(H), dtype=BF16)

@@ -1911,6 +1911,13 @@ __global__ __launch_bounds__(DEEP_THREADS) __attribute__((amdgpu_waves_per_eu(2,
     GemmArgs a) {
     gemm_pipe_body<BN, 2, 2, true, false, 64, 128, false, false, DEEP_NS, DEEP_LW>(a);
 }
+// row statistics of h W^T (ta_lm_head_logp) where a grid has at most one 128 x
+// 128 tile per CU
+template <int BN>
+__global__ __launch_bounds__(DEEP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_gemm_deep_lse(
+    GemmArgs a) {
+    gemm_pipe_body<BN, 2, 2, false, false, 64, 128, false, false, DEEP_NS, DEEP_LW, false, true>(a);
+}
 // split-K F32 partials (grid z = splits), reduced by splitk_reduce
 template <int BN, bool YT = false>
 __global__ __launch_bounds__(DEEP_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_gemm_deep_part(
@@ -3341,6 +3348,10 @@ int lm_head_logp(const bf16* h, int64_t ldh, const bf16* W, int64_t ldw, const i
     const dim3 grid(a.tiles_m * a.tiles_n);
     if (bt == 256)
         tlaunch(k_gemm_pipe_lse<256, 2, 4>, grid, dim3(512), s, a);
+    else if (pipe && a.tiles_m * a.tiles_n <= 256)
+        // (64 x 8000 x 3584 56 -> 37 us, 64 x 32,000 x 1536 35 -> 29; past one
+        // tile per CU the other way, 64 x 50,257 x 1536 43, here 47)
+        tlaunch(k_gemm_deep_lse<128>, grid, dim3(DEEP_THREADS), s, a);
     else if (pipe)
         tlaunch(k_gemm_mid_lse<128>, grid, dim3(256), s, a);
     else

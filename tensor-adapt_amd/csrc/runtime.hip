@@ -45,7 +45,7 @@ struct Scratch {
     size_t bytes = 0;
 };
 static std::mutex g_scratch_mu;
-constexpr int kSlots = 4;  // 0: partials of splits and reductions, 2: attention dK/dV partials; 1, 3: spare
+constexpr int kSlots = 4;  // 0: partials of splits and reductions, 1: softmax statistics, 2: attention dK/dV partials; 3: spare
 struct ScratchSet {
     Scratch slot[kSlots];
 };
@@ -85,7 +85,7 @@ int scratch_here(const char* what, size_t bytes, hipStream_t s, void** p) {
         TA_REQUIRE(own == dev, "%s: the stream is of device %d, the current one is %d", what, own,
                    dev);
     }
-    *p = scratch_get(bytes, s);
+    *p = scratch_get(bytes, s, 1);
     if (!*p) return set_error(-2, "%s: scratch allocation of %zu bytes failed", what, bytes);
     return 0;
 }

@@ -17,8 +17,9 @@
 namespace ta {
 
 void* scratch_get(size_t bytes, hipStream_t s, int slot = 0);
-// scratch_get with its error, also where s is not of the current device, whose
-// pool would be the wrong one
+// scratch_get of the slot of softmax statistics (which never moves the slot
+// that captured GEMMs hold), with its error, also where s is not of the current
+// device, whose pool would be the wrong one
 int scratch_here(const char* what, size_t bytes, hipStream_t s, void** p);
 // whether s records a graph (also where the runtime refuses to say)
 bool is_capturing(hipStream_t s);

@@ -804,3 +804,34 @@ def test_long_rows_captured_and_eager(N, V):
         for k in (0, 3):
             close(outs[1][k], outs[0][k].double(), 2 * sum_tol(V) + 1e-6 * outs[0][k].abs(), "logp")
         close(ds[1], ds[0].double(), ds[0].double().abs() * 2.0 ** -6 + 1e-9, "dlogits")
+
+
+def test_eager_scoring_between_replays_of_a_captured_product():
+    """The scratch of scoring is not the one that a captured split-K product
+    holds: growing it leaves the graph's replays right."""
+    M, N, K = 64, 896, 9728
+    g = gen(14)
+    X, Y = randn(g, M, K, dtype=BF16), randn(g, N, K, dtype=BF16)
+    C, want = torch.zeros(M, N, device=DEV, dtype=BF16), torch.zeros(M, N, device=DEV, dtype=BF16)
+    st = torch.cuda.Stream()
+
+    def product(out):
+        call("ta_gemm_rm", 1, 1, M, N, K, F(1), P(X), K, P(Y), K, F(0), P(out), N, None, S())
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        product(want)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=st):
+        product(C)
+    for V in (20000, 60000, 151936):
+        h, W, t = randn(g, 300, 64, dtype=BF16), randn(g, V, 64, dtype=BF16), tokens(g, 300, V, 0.1)
+        o = [full(300) for _ in range(3)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            call("ta_lm_head_logp", P(h), 64, P(W), 64, P(t), F(1), 0, *map(P, o), 300, V, 64, None,
+                 S())
+            C.zero_()
+            gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(C, want) and all(torch.isfinite(v).all() for v in o)

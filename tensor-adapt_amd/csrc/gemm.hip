@@ -229,7 +229,8 @@ __device__ __forceinline__ LseRows lse_rows(const GemmArgs& a, int BM) {
 // log2(e), lora_r bit 0: logits rounded to BF16 first, bit 1: u too, ce_lse2 and
 // lora_u[0] see lse_rows.
 // A lane holds a row's 16 TN columns of its wave, the lane 32 on the others;
-// the WNW waves of a row meet in red (LDS, [WNW][BM]).
+// the WNW waves of a row meet in red (LDS, [WNW][BM]).  (The deep form's loading
+// waves have ended by then: a barrier waits for the waves that have not.)
 template <int TM, int TN, int BM, int WNW, int NT>
 __device__ __forceinline__ void lse_tile(floatx16 (&acc)[TM][TN], const GemmArgs& a, int M,
                                          int m0, int n0, int wrow, int wn, int tn_i, int lane,
@@ -1863,7 +1864,11 @@ __global__ __launch_bounds__(WMW * WNW * 64) __attribute__((amdgpu_waves_per_eu(
     WMW * WNW / 4, WMW * WNW / 4))) void k_gemm_pipe_ce(GemmArgs a) {
     gemm_pipe_body<BN, WMW, WNW, false, false, 64, 256, true>(a);
 }
-// Row statistics of h W^T (ta_lm_head_logp) in 256 x 256 and 128 x 128 tiles.
+// Row statistics of h W^T (ta_lm_head_logp) in 256 x 256 and 128 x 128 tiles:
+// the plain kernels' main loops, an epilogue of one exponential per logit and
+// 12 bytes per row.  Bound by the MFMAs as those (8192 x 151,936 x 1536 3.1 ms,
+// 1.22 PFLOP/s), up to 128 rows by the read of W (128 x 151,936 x 896 58 us,
+// 4.7 TB/s).
 template <int BN, int WMW, int WNW>
 __global__ __launch_bounds__(WMW * WNW * 64) __attribute__((amdgpu_waves_per_eu(
     WMW * WNW / 4, WMW * WNW / 4))) void k_gemm_pipe_lse(GemmArgs a) {

@@ -106,7 +106,10 @@ __device__ __forceinline__ SoftRow span_soft(bool nt, const T* L, const Span& sp
               : span_soft_ld<T, NW, ENT, false>(L, sp, c2, redm, red);
 }
 
-// One row per block.
+// One row per block, each thread's statistics of its vectors joined at the
+// end: one read of the rows that have a token, and bound by that (4096 x 151,936
+// with 40% of the rows without one: 126 us, 5.8 TB/s).  Holding the row in
+// registers gained nothing here: there is no second pass to save.
 template <typename T, int NW, bool ENT>
 __global__ __launch_bounds__(64 * NW) void k_token_logp(const T* __restrict__ logits, int64_t ld,
                                                         const int32_t* __restrict__ targets,
@@ -427,6 +430,10 @@ struct RegRow {
     }
 };
 
+// The policy step of one row, read once and written once: statistics, loss and
+// dlogp of the token by one thread, gradient.  Bound by the two streams (2048 x
+// 151,936, a quarter of the rows without a token, KL term and entropy: 234 us,
+// 4.4 TB/s, 0.95 of a large copy's rate).
 template <int CPT, int NT, bool ENT>
 __global__ __launch_bounds__(NT) void k_policy_reg(PolicyRows r, PolicyArgs a) {
     __shared__ float redm[NT / 64];
@@ -468,7 +475,8 @@ __global__ __launch_bounds__(NT) void k_policy_reg(PolicyRows r, PolicyArgs a) {
 }
 
 // ── few rows: each over several blocks ──────────────────────────────────
-// See row_splits; part [N][splits] statistics.
+// See row_splits; part [N][splits] statistics.  One row of 151,936: 3.6 us for
+// the parts and 2.2 to join them, where one block draws the row in 11.
 template <typename T, bool ENT>
 __global__ __launch_bounds__(512) void k_soft_part(const T* __restrict__ logits, int64_t ld,
                                                    const int32_t* __restrict__ targets,
@@ -612,7 +620,9 @@ struct Tok4 {
     typedef T V __attribute__((ext_vector_type(4), aligned(4)));
 };
 // One block of NW waves per pair: half of them sum the chosen answer, half
-// the rejected one, then the loss, then the gradient.
+// the rejected one, then the loss, then the gradient.  Bound by latency: a
+// launch, one or a few loads in a row, the loss of one thread (4 pairs of 300
+// tokens 3.7 us, where an empty launch takes 2.9).
 template <int NW>
 __global__ __launch_bounds__(64 * NW) void k_preference(PrefArgs a) {
     constexpr int NH = NW / 2, NT = 64 * NH;
@@ -679,7 +689,9 @@ __global__ __launch_bounds__(64 * NW) void k_preference(PrefArgs a) {
 }
 
 // at most this many blocks of a launch over rows (its threads stay below 2^32)
-static inline dim3 row_grid(int64_t rows) { return dim3((unsigned)(rows < (1 << 20) ? rows : 1 << 20)); }
+static inline dim3 row_grid(int64_t rows) {
+    return dim3((unsigned)std::min<int64_t>(rows, 1 << 20));
+}
 constexpr int kMaxV = 1 << 30;  // indices into a row stay below 2^31
 static bool temp_ok(float c) { return c > 0.f && c < INFINITY; }
 
@@ -715,8 +727,8 @@ static int grad_splits(int N, int V, int es) {
 template <typename T>
 static int token_logp_fwd(const T* logits, int64_t ld, const int32_t* targets, float c, float* logp,
                           float* lse, float* entropy, int N, int V, hipStream_t s) {
-    TA_REQUIRE(N >= 0 && V > 0 && V <= kMaxV && ld >= V, "token_logp_fwd: bad shape N=%d V=%d ld=%lld", N, V,
-               (long long)ld);
+    TA_REQUIRE(N >= 0 && V > 0 && V <= kMaxV && ld >= V,
+               "token_logp_fwd: bad shape N=%d V=%d ld=%lld", N, V, (long long)ld);
     TA_REQUIRE(temp_ok(c), "token_logp_fwd: inv_temp must be positive and finite");
     if (N == 0) return 0;
     TA_REQUIRE(logits && targets && logp && lse, "token_logp_fwd: null argument");

@@ -416,15 +416,17 @@ struct RegRow {
         m = block_maxf<NT / 64>(m, redm);
         const float R = soft_ref(m);
         float s = 0.f, u = 0.f;
-        auto add = [&](float x) {
+        auto add = [&](float x, float& s) {
             const float d = x - R, p = __builtin_amdgcn_exp2f(d * c2);
             s += p;
             if (ENT) u = fmaf(p, fmaxf(d, kFar), u);
         };
-        if (tail >= 0) add(ft);
+        if (tail >= 0) add(ft, s);
         each([&](const float* x, int, int) {
+            float sv = 0.f;
 #pragma unroll
-            for (int e = 0; e < E; e++) add(x[e]);
+            for (int e = 0; e < E; e++) add(x[e], sv);
+            s += sv;
         });
         return block_sums<NT / 64, ENT>(m, s, u, red);
     }

@@ -28,7 +28,8 @@ __device__ __forceinline__ Soft soft_merge(const Soft& a, const Soft& b, float c
     return {M, a.s * fa + b.s * fb,
             fa * (a.u + a.s * fmaxf(da, kFar)) + fb * (b.u + b.s * fmaxf(db, kFar))};
 }
-// n values f into st; ENT: u too
+// n values f into st; ENT: u too.  S is joined from the n values' own sum: added
+// one by one they would round n times beside what may be nearly all of S.
 template <int n, bool ENT>
 __device__ __forceinline__ void soft_add(Soft& st, const float* f, float c2) {
     float gm = f[0];
@@ -41,12 +42,14 @@ __device__ __forceinline__ void soft_add(Soft& st, const float* f, float c2) {
         st.m = gm;
     }
     const float R = soft_ref(st.m);
+    float s = 0.f;
 #pragma unroll
     for (int e = 0; e < n; e++) {
         const float d = f[e] - R, p = __builtin_amdgcn_exp2f(d * c2);
-        st.s += p;
+        s += p;
         if (ENT) st.u = fmaf(p, fmaxf(d, kFar), st.u);
     }
+    st.s += s;
 }
 // Row statistics: S and U in 64 bits, since a sequence adds up the errors of
 // its rows' log S and the KL term divides them by small differences.

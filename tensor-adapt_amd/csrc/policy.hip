@@ -84,10 +84,14 @@ __device__ __forceinline__ Span span_of(int V, int z, int splits) {
 
 // statistics of a span over a block of NW waves
 template <typename T, int NW, bool ENT, bool NT>
-__device__ __forceinline__ SoftRow span_soft_ld(const T* L, const Span& sp, float c2, float* redm,
-                                                double (*red)[2]) {
+__device__ __forceinline__ SoftRow span_soft_ld(const T* L, const Span& sp, const ExpScale& c2,
+                                                float* redm, double (*red)[2]) {
     constexpr int E = Row<T>::E;
     Soft st = {-INFINITY, 0.f, 0.f};
+    // (BF16: two vectors in flight a thread, us: 4096 x 151,936 137 -> 134; not for
+    // F32 vectors, half as much work each: rows of 50,257 67.4 -> 69.2)
+    constexpr int U = E == 8 ? 2 : 1;
+#pragma unroll U
     for (int k = sp.k0 + (int)threadIdx.x; k < sp.k1; k += 64 * NW) {
         float f[E];
         Row<T>::unpack(Row<T>::template ld<NT>(L + (int64_t)k * E), f);
@@ -97,10 +101,10 @@ __device__ __forceinline__ SoftRow span_soft_ld(const T* L, const Span& sp, floa
         const float f = Row<T>::one(L + i);
         soft_add<1, ENT>(st, &f, c2);
     }
-    return soft_block<NW, ENT>(st, c2, redm, red);
+    return soft_block<NW, ENT>(st, c2.near, redm, red);
 }
 template <typename T, int NW, bool ENT>
-__device__ __forceinline__ SoftRow span_soft(bool nt, const T* L, const Span& sp, float c2,
+__device__ __forceinline__ SoftRow span_soft(bool nt, const T* L, const Span& sp, const ExpScale& c2,
                                              float* redm, double (*red)[2]) {
     return nt ? span_soft_ld<T, NW, ENT, true>(L, sp, c2, redm, red)
               : span_soft_ld<T, NW, ENT, false>(L, sp, c2, redm, red);
@@ -113,7 +117,8 @@ __device__ __forceinline__ SoftRow span_soft(bool nt, const T* L, const Span& sp
 template <typename T, int NW, bool ENT>
 __global__ __launch_bounds__(64 * NW) void k_token_logp(const T* __restrict__ logits, int64_t ld,
                                                         const int32_t* __restrict__ targets,
-                                                        float c, float* __restrict__ logp,
+                                                        float c, ExpScale c2,
+                                                        float* __restrict__ logp,
                                                         float* __restrict__ lse,
                                                         float* __restrict__ entropy, int N, int V,
                                                         bool nt) {
@@ -125,7 +130,7 @@ __global__ __launch_bounds__(64 * NW) void k_token_logp(const T* __restrict__ lo
         RowOut o = {0.0, 0.f, 0.f};
         if (t >= 0) {
             const T* L = logits + n * ld;
-            const SoftRow st = span_soft<T, NW, ENT>(nt, L, sp, c * kLog2e, redm, red);
+            const SoftRow st = span_soft<T, NW, ENT>(nt, L, sp, c2, redm, red);
             if (threadIdx.x == 0) o = row_out(st, t < V ? Row<T>::one(L + t) : 0.f, t < V, c);
         }
         if (threadIdx.x == 0) {
@@ -294,6 +299,7 @@ struct PolicyRows {
     int64_t ld;
     const int32_t* targets;
     float c;
+    ExpScale c2;
     float *logp, *entropy, *loss, *kl;
     bf16* dlogits;
     int64_t ldd;
@@ -340,7 +346,7 @@ __global__ __launch_bounds__(512) void k_policy_logits(PolicyRows r, PolicyArgs 
         if (w != 0.f) {
             const int t = r.targets[n];
             const float ft = t < r.V ? bf2f(L[t]) : 0.f;
-            const SoftRow st = span_soft<bf16, 8, ENT>(r.nt, L, sp, r.c * kLog2e, redm, red);
+            const SoftRow st = span_soft<bf16, 8, ENT>(r.nt, L, sp, r.c2, redm, red);
             if (threadIdx.x == 0) sg = policy_row(r, a, n, st, ft, w);
             __syncthreads();
             span_grad(r.nt, L, D, sp, sg, threadIdx.x, 512);
@@ -407,7 +413,7 @@ struct RegRow {
         }
     }
     template <bool ENT>
-    __device__ __forceinline__ SoftRow soft(float c2, float* redm, double (*red)[2]) {
+    __device__ __forceinline__ SoftRow soft(const ExpScale& c2, float* redm, double (*red)[2]) {
         float m = tail >= 0 ? ft : -INFINITY;
         each([&](const float* x, int, int) {
 #pragma unroll
@@ -416,16 +422,16 @@ struct RegRow {
         m = block_maxf<NT / 64>(m, redm);
         const float R = soft_ref(m);
         float s = 0.f, u = 0.f;
-        auto add = [&](float x, float& s) {
+        auto add = [&](float x, float& s, float c2) {
             const float d = x - R, p = __builtin_amdgcn_exp2f(d * c2);
             s += p;
             if (ENT) u = fmaf(p, fmaxf(d, kFar), u);
         };
-        if (tail >= 0) add(ft, s);
+        if (tail >= 0) add(ft, s, c2.near);
         each([&](const float* x, int, int) {
             float sv = 0.f;
 #pragma unroll
-            for (int e = 0; e < E; e++) add(x[e], sv);
+            for (int e = 0; e < E; e++) add(x[e], sv, c2.c[e]);
             s += sv;
         });
         return block_sums<NT / 64, ENT>(m, s, u, red);
@@ -456,7 +462,7 @@ __global__ __launch_bounds__(NT) void k_policy_reg(PolicyRows r, PolicyArgs a) {
     row.load(L, r.V, r.nt);
     const int t = r.targets[n];
     const float ft = t < r.V ? bf2f(L[t]) : 0.f;
-    const SoftRow st = row.template soft<ENT>(r.c * kLog2e, redm, red);
+    const SoftRow st = row.template soft<ENT>(r.c2, redm, red);
     if (threadIdx.x == 0) sg = policy_row(r, a, n, st, ft, w);
     __syncthreads();
     const GradRow g = uniform_row(sg);
@@ -482,7 +488,7 @@ __global__ __launch_bounds__(NT) void k_policy_reg(PolicyRows r, PolicyArgs a) {
 template <typename T, bool ENT>
 __global__ __launch_bounds__(512) void k_soft_part(const T* __restrict__ logits, int64_t ld,
                                                    const int32_t* __restrict__ targets,
-                                                   const float* __restrict__ weight, float c2,
+                                                   const float* __restrict__ weight, ExpScale c2,
                                                    SoftRow* __restrict__ part, int V, int splits) {
     __shared__ float redm[8];
     __shared__ double red[8][2];
@@ -744,20 +750,21 @@ static int token_logp_fwd(const T* logits, int64_t ld, const int32_t* targets, f
         const float* no_weight = nullptr;
         if (entropy) {
             tlaunch(k_soft_part<T, true>, grid, dim3(512), s, logits, ld, targets, no_weight,
-                    c * kLog2e, part, V, splits);
+                    exp_scale(c), part, V, splits);
             tlaunch(k_token_logp_join<T, true>, dim3(N), dim3(64), s, logits, ld, targets, c, part,
                     splits, logp, lse, entropy, V);
         } else {
             tlaunch(k_soft_part<T, false>, grid, dim3(512), s, logits, ld, targets, no_weight,
-                    c * kLog2e, part, V, splits);
+                    exp_scale(c), part, V, splits);
             tlaunch(k_token_logp_join<T, false>, dim3(N), dim3(64), s, logits, ld, targets, c,
                     part, splits, logp, lse, entropy, V);
         }
         return check_launch("token_logp_fwd");
     }
     const bool nt = (int64_t)N * V * (int64_t)sizeof(T) > kCacheBytes;
+    const ExpScale c2 = exp_scale(c);
 #define TL(NW, ENT)                                                                             \
-    tlaunch(k_token_logp<T, NW, ENT>, row_grid(N), dim3(64 * NW), s, logits, ld, targets, c,    \
+    tlaunch(k_token_logp<T, NW, ENT>, row_grid(N), dim3(64 * NW), s, logits, ld, targets, c, c2, \
             logp, lse, entropy, N, V, nt)
     const int nw = fwd_waves(N, V);
     if (nw == 2) {
@@ -904,7 +911,7 @@ int ta_policy_loss_logits(const uint16_t* logits, int64_t ld, const int32_t* tar
     const PolicyArgs a{old_logp, ref_logp, adv,       weight,  clip_lo,
                        clip_hi,  dual_clip, kl_beta, ent_coef};
     hipStream_t s = (hipStream_t)stream;
-    const PolicyRows r{logits, ld,   targets, inv_temp, logp, entropy,
+    const PolicyRows r{logits, ld,   targets, inv_temp, exp_scale(inv_temp), logp, entropy,
                        loss,   kl,   dlogits, ldd,      N,    V,
                        (int64_t)N * V * 2 > kCacheBytes};
     // (three launches instead of one: 1 row of 151,936 26 -> 15 us, 64 rows 30
@@ -921,11 +928,11 @@ int ta_policy_loss_logits(const uint16_t* logits, int64_t ld, const int32_t* tar
         const dim3 grid(N * splits);
         if (entropy) {
             tlaunch(k_soft_part<bf16, true>, grid, dim3(512), s, logits, ld, targets, weight,
-                    inv_temp * kLog2e, part, V, splits);
+                    exp_scale(inv_temp), part, V, splits);
             tlaunch(k_policy_join<true>, dim3(N), dim3(64), s, r, a, part, splits, grads);
         } else {
             tlaunch(k_soft_part<bf16, false>, grid, dim3(512), s, logits, ld, targets, weight,
-                    inv_temp * kLog2e, part, V, splits);
+                    exp_scale(inv_temp), part, V, splits);
             tlaunch(k_policy_join<false>, dim3(N), dim3(64), s, r, a, part, splits, grads);
         }
         tlaunch(k_policy_grad, grid, dim3(512), s, r, grads, splits);

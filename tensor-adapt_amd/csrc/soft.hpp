@@ -14,6 +14,32 @@
 
 namespace ta {
 
+// c log2(e) for the eight values of a vector.  Rounded to one F32 the factor is
+// off by up to 2^-24, the same way for every logit, and log S by that times the
+// mean of |c d|: of the sums' errors the one that does not average out, and a
+// policy near its reference shows it in the KL term.  So k of eight values take
+// the F32 above it and the others the F32 below, which leaves a sixteenth of
+// their distance at most and costs no instruction (a second product with the
+// factor's remainder made the forward 6% slower).
+struct ExpScale {
+    float c[8];
+    float near;  // the nearest F32, for single factors
+};
+inline ExpScale exp_scale(float c) {
+    const double x = (double)c * 1.44269504088896340736;
+    ExpScale r;
+    r.near = (float)fmin(x, 3.4028234663852886e38);
+    const float lo = (double)r.near > x ? nextafterf(r.near, 0.f) : r.near;
+    const float up = fminf(nextafterf(lo, INFINITY), 3.4028234663852886e38f);
+    const int k = up > lo ? (int)lrint(8 * (x - (double)lo) / ((double)up - (double)lo)) : 0;
+    // (in the order 0 4 2 6 1 5 3 7, so that the first four are near k / 8 too)
+    for (int e = 0; e < 8; e++) {
+        const int order = (e & 1) << 2 | (e & 2) | e >> 2;
+        r.c[e] = order < k || lo == 0.f ? up : lo;
+    }
+    return r;  // (none is 0: a logit of -Inf gives exp(-Inf), not 0 * -Inf)
+}
+
 // m: maximum (-Inf: none yet), s, u: the sums above relative to m, u without
 // the factor c.  c2 = c log2(e): exp(c d) = exp2(c2 d), one v_exp_f32.
 struct Soft {
@@ -31,12 +57,12 @@ __device__ __forceinline__ Soft soft_merge(const Soft& a, const Soft& b, float c
 // n values f into st; ENT: u too.  S is joined from the n values' own sum: added
 // one by one they would round n times beside what may be nearly all of S.
 template <int n, bool ENT>
-__device__ __forceinline__ void soft_add(Soft& st, const float* f, float c2) {
+__device__ __forceinline__ void soft_add(Soft& st, const float* f, const ExpScale& c2) {
     float gm = f[0];
 #pragma unroll
     for (int e = 1; e < n; e++) gm = fmaxf(gm, f[e]);
     if (gm > st.m) {
-        const float d = st.m - gm, k = __builtin_amdgcn_exp2f(d * c2);
+        const float d = st.m - gm, k = __builtin_amdgcn_exp2f(d * c2.near);
         if (ENT) st.u = k * (st.u + st.s * fmaxf(d, kFar));
         st.s *= k;
         st.m = gm;
@@ -45,7 +71,7 @@ __device__ __forceinline__ void soft_add(Soft& st, const float* f, float c2) {
     float s = 0.f;
 #pragma unroll
     for (int e = 0; e < n; e++) {
-        const float d = f[e] - R, p = __builtin_amdgcn_exp2f(d * c2);
+        const float d = f[e] - R, p = __builtin_amdgcn_exp2f(d * c2.c[e]);
         s += p;
         if (ENT) st.u = fmaf(p, fmaxf(d, kFar), st.u);
     }
